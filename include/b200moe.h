@@ -270,6 +270,74 @@ int b200moe_scaled_mm(void* out, int out_dtype, const void* a, const void* b, co
                       const float* scale_b, int64_t M, int64_t K, int64_t N, void* workspace, size_t workspace_bytes,
                       int32_t* status, void* stream);
 
+/* ---- gradients -------------------------------------------------------------------------------------------
+ * The gradients of the entry points above, for training through a layer or for fine-tuning what lies around one.  No
+ * reference counterpart (its MoE ops are inference ops).  Products with FP8 weights run on the FP8 tensor cores as in the
+ * forward call: Q(.) below quantises rows to e4m3 per 128 columns, scale = max|.| / 448 (the maximum is taken as at least 1e-12
+ * for activations and 1e-30 for gradients), and gradients pass a quantisation unchanged.  Sums are fp32.  Equal calls give
+ * equal bits, except dx of b200moe_experts_backward at T*k <= 512 (partial sums may meet in fp32 reductions there).
+ * Weight gradients are in the weights' layout, fp32 or bf16 (`*_dtype`); accumulate = 1 (fp32 only) adds them to what
+ * the buffer holds.  Experts without rows get a zero gradient.  With T = 0 only the weight gradients are written (zeros).
+ * Tensors may not overlap unless a call says so. */
+
+/* Of b200moe_route: dlogits[T,E] (fp32) from dw[T,k] (fp32 or bf16), the logits that were routed and the ids that came out.
+ * With s the scores (softmax | sigmoid of logits + logit_bias), p_j = s[ids[j]], S = sum_j p_j, c = scale:
+ *   dp_j = c * (dw_j - sum_i dw_i p_i / S) / S  with renorm,  else  c * dw_j
+ *   softmax: dlogits_e = s_e * ([e = ids[j]] dp_j - sum_i dp_i p_i);   sigmoid: dlogits_e = s_e (1 - s_e) [e = ids[j]] dp_j
+ * Selection itself (groups, bias) has no gradient.  Slots with an id outside [0,E) count for nothing.  dlogits may be the
+ * logits' own buffer.  E <= 1024, k <= 32, k <= E. */
+int b200moe_route_backward(float* dlogits, const float* logits, const float* logit_bias, const int32_t* ids, const void* dw,
+                           int dw_dtype, int64_t T, int64_t E, int64_t k, int score_func, int renorm, float scale, void* stream);
+
+/* Of b200moe_router_logits: dx[T,H] (bf16) = dlogits[T,E] . wr[E,H], dwr[E,H] = dlogits^T . x[T,H].  dlogits fp32 (taken
+ * as two bf16 numbers each, 2^-17 relative); dx or dwr may be NULL, and then wr or x too.  H % 8 == 0, E <= 1024. */
+size_t b200moe_router_logits_backward_workspace_bytes(int64_t T, int64_t H, int64_t E);
+int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype, int accumulate, const float* dlogits, const void* x,
+                                   const void* wr, int64_t T, int64_t H, int64_t E, void* workspace, size_t workspace_bytes,
+                                   int32_t* status, void* stream);
+
+/* Of b200moe_combine (b200moe_combine_masked with ids): dy[t,j,:] (bf16) = w[t,j] * dout[t,:], dw[t,j] (fp32) = <dout[t,:], y[t,j,:]>.
+ * Masked slots: dy = 0, dw = 0, y is not read.  (The gradient of `add` is dout itself.)  dy or dw may be NULL, and then w or y
+ * too.  dy may be y's own buffer.  H % 8 == 0, k <= 32. */
+int b200moe_combine_backward(void* dy, float* dw, const void* dout, const void* y, const void* w, int w_dtype,
+                             const int32_t* ids, int64_t E, int64_t T, int64_t k, int64_t H, void* stream);
+
+/* Of b200moe_linear_w8: dx[M,K] (bf16) = Q(dy) . dequant(w), dw[N,K] = dy^T . x (bf16 operands).  dy bf16 [M,N], x bf16 [M,K].  dx or
+ * dw may be NULL, and then w and scale, or x, too.  K % 128 == 0, N % 64 == 0. */
+size_t b200moe_linear_w8_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int scale_dtype);
+int b200moe_linear_w8_backward(void* dx, void* dw, int dw_dtype, int accumulate, const void* dy, const void* x, const void* w,
+                               const void* scale, int scale_dtype, int64_t M, int64_t K, int64_t N, void* workspace,
+                               size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Of b200moe_experts (FP8 weights, B200MOE_ACT_W8A8).  For the row of pair (t,j) with expert e and weight w = topk_w[t,j] (per_slot:
+ * w = 1 and dout has a row for each pair):
+ *   g = Q(x) Wg^T, u = Q(x) Wu^T, h = silu(g) * u          (formed again: nothing of the forward call is kept)
+ *   d = Q(dout) Wd                                         (Wd: the down projection, stored as w_down [I,H])
+ *   dw[t,j] = <h, d>;  dg = w d u silu'(g),  du = w d silu(g)
+ *   dx[t,:] = sum_j (Q(dg) Wg + Q(du) Wu) (+ add[t,:])      (a slot's row is rounded to bf16 before the
+ *                                                          sum, unless T*k <= 512 and K is split)
+ *   dWg = sum dg^T x,  dWu = sum du^T x,  dWd = sum (w h)^T dout   over the expert's rows; dg, du and w h rounded to bf16
+ *   dx        bf16 [T,H] or NULL           dw  fp32 [T,k] or NULL (NULL with per_slot)
+ *   dw_gate, dw_up, dw_down  [E,I,H] of grad_dtype (weight_grads = 1; else ignored)
+ *   dout      bf16 [T,H], per_slot: [T,k,H]
+ *   add       bf16 [T,H] or NULL (e.g. the router's or a shared expert's dx; may be dx's own buffer)
+ * Pairs with an id outside [0,E) contribute nothing, their dw is 0 (status bit 0).  Sizes as b200moe_experts. */
+typedef struct {
+  int64_t T, H, I, E, k;
+  int per_slot;      /* 1 = dout [T,k,H] of un-weighted rows, topk_w must be NULL */
+  int scale_dtype;   /* B200MOE_F32 | B200MOE_BF16 */
+  int w_dtype;       /* of topk_w: B200MOE_F32 | B200MOE_BF16 */
+  int weight_grads;
+  int grad_dtype;    /* of the weight gradients: B200MOE_F32 | B200MOE_BF16 */
+  int accumulate;
+} b200moe_experts_backward_desc;
+size_t b200moe_experts_backward_workspace_bytes(const b200moe_experts_backward_desc* d);
+int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void* dw_up, void* dw_down, const void* dout, const void* x,
+                             const void* w_gate, const void* w_up, const void* w_down, const void* s_gate, const void* s_up,
+                             const void* s_down, const int32_t* ids, const void* topk_w, const void* add,
+                             const b200moe_experts_backward_desc* d, void* workspace, size_t workspace_bytes, int32_t* status,
+                             void* stream);
+
 /* ---- expert parallelism over peer memory (NVLink) --------------------------------------------------
  * No reference counterpart (the reference has no expert parallelism).  One process per GPU of one node; every
  * rank allocates the same set of buffers, exports them (CUDA IPC) and imports its peers' handles, then builds

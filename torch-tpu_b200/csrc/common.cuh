@@ -16,6 +16,7 @@
 constexpr int kBlock = 128;          // quantisation block (columns per activation scale, weight tile edge)
 constexpr float kFp8Max = 448.0f;    // largest finite e4m3 value
 constexpr float kAmaxFloor = 1e-12f; // floor of a group's max|x| before the scale is formed
+constexpr float kGradAmaxFloor = 1e-30f; // the same for gradients, which may be small throughout (448 / floor stays finite)
 
 #define MOE_CHECK_ARG(cond)            \
   do {                                 \

@@ -166,6 +166,8 @@ int check_desc(const b200moe_experts_desc* d) {
 
 }  // namespace
 
+int moe_choose_ksplit(int64_t P, int64_t E, int64_t H, int64_t K) { return choose_ksplit(P, E, H, K); }
+
 extern "C" size_t b200moe_experts_workspace_bytes(const b200moe_experts_desc* d) {
   if (check_desc(d) != B200MOE_OK) return 0;
   return make_layout(*d).total;

@@ -10,6 +10,13 @@
 //          the rank that owns the token (expert parallelism over peer memory: plain peer stores)
 //   linear out = x W^T with W [N,K]      one "expert", no activation, bf16 rows out (my_ops/MmW8A16Dq.cpp:185-229)
 //
+// and the products of their gradients (no reference counterpart; formulas at b200moe_experts_backward in the header):
+//
+//   dh     d = Q(dout) Wd^T              per expert, fp32, kept in the layout that the next product's epilogue reads
+//   swiglu gate and up are formed again as in gemm1; the epilogue turns them and d into dgate and dup (e4m3 and bf16),
+//          w * h (bf16) and the row's share of the routing weight's gradient
+//   dx     y = Q(dgate) Wg + Q(dup) Wu   one K loop over both weight tensors; with one tensor the linear layer's dx
+//
 // One persistent CTA per SM, 12 warps: warp 0 = TMA producer of the weights, warp 1 = MMA issuer (one thread) and TMEM
 // owner, warp 2 = scout (walks the next work item's expert, row range and first scales and leaves them in shared
 // memory), warp 3 = TMA producer of the activations, warps 4..11 = epilogue (TMEM lane quarter = warp%4, column half = (warp-4)/4).  setmaxnreg
@@ -113,7 +120,18 @@ struct TcArgs {
   float* hs_t;
   __nv_bfloat16* out;
   int32_t* status;
+  int segs;             // MODE 4: weight tensors along K (1 or 2)
+  float* dh;            // MODE 5 writes, MODE 3 reads: d, [m-tile][I/128] blocks of 128 x 128 (see dh_index)
+  float* dwp;           // MODE 3: partial sums of h * d, [I/64][ld], or NULL
+  __nv_bfloat16* g16;   // MODE 3: bf16 rows [P, 3I] = dgate | dup | w * h, or NULL
 };
+
+// Where the 64 columns of epilogue thread (q, cg, lane) lie in a 128 x 128 block of d, in float4s: 32 lanes side by side, so
+// that both the product that writes d and the one that reads it move whole 512-byte runs without a turn through shared
+// memory.  i: four columns each.
+__device__ __forceinline__ size_t dh_index(int mt, int nI, int nt, int q, int cg, int i, int lane) {
+  return ((((size_t)mt * nI + nt) * 8 + q * 2 + cg) * 16 + i) * 32 + lane;
+}
 
 // A pair of fp32 accumulators (two scalar FMAs per pair: on this part the packed fma.rn.f32x2 form was no faster in
 // the tensor-memory read-back loop, and the scalar form leaves the register allocator free to place the pairs)
@@ -143,11 +161,13 @@ __host__ __device__ constexpr uint32_t make_idesc(int b_mn_major) {
 
 // MODE 0 = gate/up GEMM (+ SiLU*up + requantise), 1 = down GEMM, 2 = plain linear layer: out[r, :N] = A[r, :K] W^T with
 // W [N, K] K-major (the gate/up operand path with the down GEMM's bf16 store; a.I = N, a.H = K, 256 outputs per tile)
+// Gradients: 3 = swiglu (operands as 0), 4 = dx (operands as 1, K = one or two weight tensors of I rows each, the last
+// block of a tensor may be half a block), 5 = dh (operands as 2)
 template <int MODE>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs,
                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1, const TcArgs a) {
-  constexpr bool GEMM2 = MODE == 1, DENSE = MODE == 2;
+  constexpr bool GEMM2 = MODE == 1 || MODE == 4, DENSE = MODE == 2 || MODE == 5, GATE_UP = MODE == 0 || MODE == 3;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcShared* sh = reinterpret_cast<TcShared*>(smem + (size_t)TC_STAGES * TC_STAGE_BYTES);
@@ -194,10 +214,11 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   if (!a.lists_ready) pdl_wait();
 
   const int num_mtiles = *a.num_mtiles;
-  const int KB_all = (GEMM2 ? a.I : a.H) / kBlock;
+  const int KBI = (a.I + kBlock - 1) / kBlock;  // MODE 4: K blocks of one weight tensor
+  const int KB_all = MODE == 4 ? a.segs * KBI : (GEMM2 ? a.I : a.H) / kBlock;
   // work items: (n-tile, m-tile, K split); without a K split the last ones may be parts of shared tiles
   WorkPlan plan{num_mtiles * a.NT * a.KS, 1, num_mtiles * a.NT * a.KS, KB_all};
-  if (MODE != 0 && a.part) plan = work_plan(num_mtiles * a.NT, KB_all, a.plan_ctas, a.part_rows);
+  if (!GATE_UP && a.part) plan = work_plan(num_mtiles * a.NT, KB_all, a.plan_ctas, a.part_rows);
   const int total_tiles = plan.items;
   const int nH = a.H / kBlock, nI = a.I / kBlock;
 
@@ -205,7 +226,10 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   // Indices are rebuilt from a few 32-bit values every K block instead of keeping pointers alive: the epilogue
   // loop runs at the edge of the register file and a spilled value costs an L2 round trip here.
   const float* const S0 = reinterpret_cast<const float*>(a.s0);
-  const float* const S1 = (GEMM2 || DENSE) ? S0 : reinterpret_cast<const float*>(a.s1);  // one scale tensor
+  // one scale tensor, or (MODE 4) a second one whose K blocks follow the first's
+  const float* const S1 = MODE == 4 ? reinterpret_cast<const float*>(a.s1) - (int64_t)KBI * (a.H / kBlock)
+                          : (GEMM2 || DENSE) ? S0 : reinterpret_cast<const float*>(a.s1);
+  auto scales_of = [&](int half, int kb) { return MODE == 4 ? (kb >= KBI ? S1 : S0) : half ? S1 : S0; };  // kb: K block of the whole range
   const int sstep = GEMM2 ? nH : 1;
   const int nIs = (a.I + kBlock - 1) / kBlock;  // scale rows of one expert (= nI unless a linear layer's N % 128 != 0)
   struct Item {
@@ -214,7 +238,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   auto item_of = [&](int t) {
     Item w;
     int ks = 0, tt = t;
-    if (MODE != 0 && a.part) {
+    if (!GATE_UP && a.part) {
       const WorkItem i = work_item(plan, t);
       tt = i.tile, w.kb0 = i.kb0, w.KB = i.KB;
     } else {
@@ -222,18 +246,18 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     }
     w.nt = a.m_major ? tt % a.NT : tt / num_mtiles;
     w.mt = a.m_major ? tt / a.NT : tt - w.nt * num_mtiles;
-    if (MODE != 0 && a.part) return w;
+    if (!GATE_UP && a.part) return w;
     w.kb0 = (int)((int64_t)KB_all * ks / a.KS);
     w.KB = (int)((int64_t)KB_all * (ks + 1) / a.KS) - w.kb0;  // K blocks of this work item
     return w;
   };
   // (32-bit: the launcher refuses scale tensors of 2^31 elements or more)
   auto scale_index = [&](const Item& w, int e, int& w0i, int& w1i) {
-    w0i = (GEMM2 ? e * nI * nH + 2 * w.nt : DENSE ? (e * nIs + 2 * w.nt) * nH : (e * nI + w.nt) * nH) + w.kb0 * sstep;
+    w0i = (GEMM2 ? e * (MODE == 4 ? KBI : nI) * nH + 2 * w.nt : DENSE ? (e * nIs + 2 * w.nt) * nH : (e * nI + w.nt) * nH) + w.kb0 * sstep;
     w1i = w0i + (GEMM2 ? ((2 * w.nt + 1 < nH) ? 1 : 0) : DENSE ? ((2 * w.nt + 1 < nIs) ? nH : 0) : 0);
   };
   // results are bf16 rows stored to row_map / row_src destinations (uniform over the launch)
-  const bool rows_out = MODE != 0 && (a.row_src || (a.KS == 1 && !a.comb32 && !(DENSE && a.out32)));
+  const bool rows_out = !GATE_UP && MODE != 5 && (a.row_src || (a.KS == 1 && !a.comb32 && !(DENSE && a.out32)));
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_REG_LO));
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer of the weights (one thread)
@@ -256,13 +280,21 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
         const int KB = nx.KB;
         // coordinates of the two boxes of the first K block, and their step per K block
+        const int kb0 = nx.kb0;
         const int n0 = nx_e * a.I + (GEMM2 ? nx.kb0 * kBlock : nx.nt * (DENSE ? 256 : 128));  // row of the weight matrix
         const int c0 = GEMM2 ? nx.nt * 256 : nx.kb0 * kBlock;
+        const int first_row = nx_e * a.I;
         if (t + (int)gridDim.x < total_tiles) {
           nx = item_of(t + gridDim.x);
           nx_e = a.mtiles[2 * nx.mt];
         }
         int row = n0, col = c0;
+        const CUtensorMap* tmB = &tmB0;
+        int left = 0;  // MODE 4: K blocks of the first weight tensor that are still to come
+        if (MODE == 4) {
+          left = KBI - kb0;
+          if (left <= 0) tmB = &tmB1, row -= KBI * kBlock;
+        }
         for (int kb = 0; kb < KB; ++kb) {
           const uint32_t full = smem_u32(&sh->full[0]) + s * 8, sb = smem_base + TC_A_BYTES + s * TC_STAGE_BYTES;
           if (ahead-- == 0) pdl_wait();
@@ -271,8 +303,9 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             break;
           }
           mbar_arrive_expect_tx(full, TC_B_BYTES);
-          tma_load_2d(sb, &tmB0, col, row, full);
-          if (GEMM2) tma_load_2d(sb + 128 * 128, &tmB0, col + 128, row, full);
+          if (MODE == 4 && left-- == 0) tmB = &tmB1, row = first_row;
+          tma_load_2d(sb, tmB, col, row, full);
+          if (GEMM2) tma_load_2d(sb + 128 * 128, tmB, col + 128, row, full);
           else tma_load_2d(sb + 128 * 128, DENSE ? &tmB0 : &tmB1, col, row + (DENSE ? 128 : 0), full);
           if (GEMM2) row += kBlock;
           else col += kBlock;
@@ -291,7 +324,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                                     : make_smem_desc(smem_base + TC_A_BYTES, 16, 1024);
       uint32_t n_it = 0;
       for (int t = blockIdx.x; t < total_tiles; t += gridDim.x) {
-        if (MODE != 0 && a.part) {
+        if (!GATE_UP && a.part) {
           n_it += (uint32_t)work_item(plan, t).KB;
         } else {
           const int ks = t % a.KS;
@@ -349,7 +382,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         }
       }
       float wv = 0.f;  // lanes 0..3: S0[w0i], S1[w1i], S0[w0i + sstep], S1[w1i + sstep]
-      if (lane < 2 || (lane < 4 && w.KB > 1)) wv = ((lane & 1) ? S1 : S0)[((lane & 1) ? w1i : w0i) + ((lane >> 1) ? sstep : 0)];
+      if (lane < 2 || (lane < 4 && w.KB > 1)) wv = scales_of(lane & 1, w.kb0 + (lane >> 1))[((lane & 1) ? w1i : w0i) + ((lane >> 1) ? sstep : 0)];
       // the slot is free once every epilogue warp has taken item n - 1 out of it
       if (n > 0 && !mbar_wait(smem_u32(&sh->head_empty), (n - 1) & 1, abort_flag)) {
         ok = false;
@@ -358,6 +391,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       if (lane == 0) {
         sh->head_item[0] = e, sh->head_item[1] = row0, sh->head_item[2] = row_end;
         sh->head_item[3] = w.nt, sh->head_item[4] = w.kb0, sh->head_item[5] = w.KB;
+        if (MODE == 3 || MODE == 5) sh->head_item[6] = w.mt;
       }
       if (lane < 4) sh->head_w[lane] = wv;
 #pragma unroll
@@ -448,6 +482,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       if (ok) {
         e = sh->head_item[0], row0 = sh->head_item[1], row_end = sh->head_item[2];
         w.nt = sh->head_item[3], w.kb0 = sh->head_item[4], w.KB = sh->head_item[5];
+        if (MODE == 3 || MODE == 5) w.mt = sh->head_item[6];
         // Scale factors f0 = sa[row,kb] * sw_gate[kb], f1 = sa[row,kb] * sw_up[kb]: the products of block kb + 1 are
         // formed and the values of block kb + 2 are requested while block kb's TMEM loads are in flight.
         const float sa0 = sh->head_sa[0][rit];
@@ -460,6 +495,8 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const int grow = row0 + rit;
       const bool valid = grow < row_end;
       const bool warp_has_rows = row0 + q * 32 < row_end;  // uniform over the warp
+      float row_w = 1.f;  // MODE 3: the row's routing weight
+      if (MODE == 3 && a.comb_w && valid) row_w = moe_load_as_f32(a.comb_w, a.row_map[grow], a.comb_wdt);
       int w0i, w1i;
       scale_index(w, e, w0i, w1i);
       // accumulators as packed fp32 pairs: acc[j][p] = columns (2p, 2p+1) of this thread's TC_CW-column span of half j
@@ -517,8 +554,8 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           const float nf0 = sa1 * wa1, nf1 = sa1 * wb1;  // block kb + 1
           if (kb + 2 < KB) {
             sa1 = load_sa(kb + 2);
-            wa1 = S0[w0i + (kb + 2) * sstep];
-            wb1 = S1[w1i + (kb + 2) * sstep];
+            wa1 = scales_of(0, kb0 + kb + 2)[w0i + (kb + 2) * sstep];
+            wb1 = scales_of(1, kb0 + kb + 2)[w1i + (kb + 2) * sstep];
           }
           tc_ld_wait(s0, s1);
 #pragma unroll
@@ -563,7 +600,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       } else {
         clear_acc();  // (a wait ran out: nothing below stores anything, but nothing reads an unset register either)
       }
-      if (MODE != 0 && t >= plan.whole) {
+      if (!GATE_UP && t >= plan.whole) {
         // A part of a shared tile (a CTA of the whole grid has one at most, its last item; one of a capped grid can have
         // several): the partial sums go to the part's slot (16 bytes per lane, consecutive over the warp; only rows that
         // exist), the CTA counts itself in, and the one that comes last adds the parts up in K order - the order of the
@@ -615,6 +652,119 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         }
       }
       float amax = 0.f;
+      if constexpr (MODE == 3) {
+        // gate, up, d -> dgate = w d up s (1 + gate (1 - s)), dup = w d gate s, h = gate s up with s = sigmoid(gate), all in
+        // fp32 from the accumulators; dgate and dup overwrite gate and up.  Then, per row and 128 columns, dgate and dup
+        // are quantised like every operand (the two column-half warps exchange their maxima as in MODE 0).
+        const int nI3 = a.I / kBlock, wepi = warp - 4;
+        uint4* wst = reinterpret_cast<uint4*>(sh->ostage + 4096 + wepi * 2048);  // 32 rows x 64 B, past the row maxima
+        // the patch's 32 rows to row-segment stores of 64 bytes: base + row * stride + byte offset
+        auto store_patch = [&](uint8_t* base, int64_t stride, int64_t at) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // 8 rows x 64 B per instruction
+            const int r = i * 8 + (lane >> 2), c = lane & 3;
+            const int orow = row0 + q * 32 + r;
+            if (orow < row_end)
+              *reinterpret_cast<uint4*>(base + orow * stride + at + c * 16) = wst[r * 4 + (c ^ ((r >> 1) & 3))];
+          }
+          __syncwarp();
+        };
+        auto pack_bf16 = [](float x, float y) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+          return *reinterpret_cast<const uint32_t*>(&v);
+        };
+        uint8_t* const g16 = reinterpret_cast<uint8_t*>(a.g16);
+        const int64_t g16_stride = (int64_t)a.I * 6, col = nt * 128 + cg * TC_CW;
+        float amax_u = 0.f, dot = 0.f;
+        const float4* dsrc = reinterpret_cast<const float4*>(a.dh);
+        if (warp_has_rows && ok) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {  // 32 columns each
+            float4 dv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dv[i] = valid ? __ldcg(dsrc + dh_index(w.mt, nI3, nt, q, cg, half * 8 + i, lane)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int v4 = 0; v4 < 4; ++v4) {
+              uint32_t ow[4];
+#pragma unroll
+              for (int w4 = 0; w4 < 4; ++w4) {
+                const int i = half * 16 + v4 * 4 + w4;  // pair of columns
+                const float4 d4 = dv[v4 * 2 + (w4 >> 1)];
+                const float2 g = unpack2(acc[0][i]), u = unpack2(acc[1][i]);
+                const float d[2] = {(w4 & 1) ? d4.z : d4.x, (w4 & 1) ? d4.w : d4.y}, gg[2] = {g.x, g.y}, uu[2] = {u.x, u.y};
+                float dg[2], du[2], hw[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const float sg = __fdividef(1.f, 1.f + __expf(-gg[c]));
+                  const float act = gg[c] * sg, h = act * uu[c], dd = row_w * d[c];
+                  dot = fmaf(h, d[c], dot);
+                  dg[c] = dd * uu[c] * fmaf(act, 1.f - sg, sg);
+                  du[c] = dd * act;
+                  hw[c] = row_w * h;
+                }
+                acc[0][i] = pack2(dg[0], dg[1]);
+                acc[1][i] = pack2(du[0], du[1]);
+                amax = fmaxf(amax, fmaxf(fabsf(dg[0]), fabsf(dg[1])));
+                amax_u = fmaxf(amax_u, fmaxf(fabsf(du[0]), fabsf(du[1])));
+                ow[w4] = pack_bf16(hw[0], hw[1]);
+              }
+              if (g16) wst[lane * 4 + (v4 ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+            }
+            if (g16) store_patch(g16, g16_stride, (int64_t)a.I * 4 + (col + half * 32) * 2);
+          }
+          if (valid && a.dwp) a.dwp[(int64_t)(nt * TC_CG + cg) * a.ld + grow] = dot;
+        }
+        float* const maxima = reinterpret_cast<float*>(sh->ostage) + (ntile & 1) * (2 * TC_CG * 128);  // [tensor][column half][row]
+        maxima[cg * 128 + rit] = amax;
+        maxima[(TC_CG + cg) * 128 + rit] = amax_u;
+        if (epi_any(!ok)) {
+          ok = false;
+          break;
+        }
+        if (warp_has_rows) {
+#pragma unroll
+          for (int o = 0; o < TC_CG; ++o) {
+            amax = fmaxf(amax, maxima[o * 128 + rit]);
+            amax_u = fmaxf(amax_u, maxima[(TC_CG + o) * 128 + rit]);
+          }
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const float top = fmaxf(m ? amax_u : amax, kGradAmaxFloor);
+            const float inv = kFp8Max / top;
+            if (valid && cg == 0) a.hs_t[(int64_t)(m * nI3 + nt) * a.ld + grow] = top / kFp8Max;
+#pragma unroll
+            for (int v4 = 0; v4 < TC_CW / 16; ++v4) {
+              uint32_t ow[4];
+#pragma unroll
+              for (int w4 = 0; w4 < 4; ++w4) {
+                const float2 p0 = unpack2(acc[m][v4 * 8 + w4 * 2]), p1 = unpack2(acc[m][v4 * 8 + w4 * 2 + 1]);
+                ow[w4] = moe_f32x4_to_e4m3x4(p0.x * inv, p0.y * inv, p1.x * inv, p1.y * inv);
+              }
+              wst[lane * 4 + (v4 ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+            }
+            store_patch(a.hq, (int64_t)a.I * 2, (int64_t)m * a.I + col);
+            if (g16) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int v4 = 0; v4 < 4; ++v4) {
+                  uint32_t ow[4];
+#pragma unroll
+                  for (int w4 = 0; w4 < 4; ++w4) {
+                    const float2 v = unpack2(acc[m][half * 16 + v4 * 4 + w4]);
+                    ow[w4] = pack_bf16(v.x, v.y);
+                  }
+                  wst[lane * 4 + (v4 ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+                }
+                store_patch(g16, g16_stride, (int64_t)m * a.I * 2 + (col + half * 32) * 2);
+              }
+            }
+          }
+        }
+        continue;
+      }
       if (MODE == 0) {
         // SiLU(gate) * up; the row's 128 values are split over TC_CG warps, which exchange their maxima through
         // shared memory (two copies, alternating by tile, so that one barrier per tile is enough)
@@ -639,7 +789,23 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       // shared memory instead (16-byte chunks, XOR-swizzled so that neither side has bank conflicts; only warp-level
       // synchronisation) and then stores whole 64- or 128-byte row segments per group of lanes.  (Handing each row's
       // 128 bytes to the copy engine, so that the warp could go on, was slower: Qwen3 down GEMM 196 -> 241 us.)
-      static_assert(TC_CW == 64, "the row-segment stores below are laid out for 64 columns per warp");
+      static_assert(TC_CW == 64, "the row-segment stores are laid out for 64 columns per warp");
+      if constexpr (MODE == 5) {
+        const int nI5 = a.I / kBlock;
+        float4* dst = reinterpret_cast<float4*>(a.dh);
+        if (valid) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (2 * nt + j < nI5) {
+#pragma unroll
+              for (int i = 0; i < TC_CW / 4; ++i) {
+                const float2 p0 = unpack2(acc[j][i * 2]), p1 = unpack2(acc[j][i * 2 + 1]);
+                __stcg(dst + dh_index(w.mt, nI5, 2 * nt + j, q, cg, i, lane), make_float4(p0.x, p0.y, p1.x, p1.y));
+              }
+            }
+        }
+        continue;
+      }
       const int wepi = warp - 4;
       if (MODE == 0) {
 #pragma unroll
@@ -818,20 +984,24 @@ int device_sm_count() {
 
 template <int MODE>
 int launch_tc(const MoeGemmArgs& g, cudaStream_t st) {
-  constexpr bool GEMM2 = MODE == 1, DENSE = MODE == 2;
+  constexpr bool GEMM2 = MODE == 1 || MODE == 4, DENSE = MODE == 2 || MODE == 5, GATE_UP = MODE == 0 || MODE == 3;
   if (g.scale_dtype != B200MOE_F32) return B200MOE_EINVAL;  // the caller converts bf16 scales first
   if ((int64_t)g.E * ((g.I + kBlock - 1) / kBlock) * (g.H / kBlock) >= (int64_t(1) << 31)) return B200MOE_EINVAL;  // 32-bit scale indices
-  const int K = GEMM2 ? g.I : g.H;
+  const int K = MODE == 4 ? g.segs * g.I : GEMM2 ? g.I : g.H;
   CUtensorMap tmA, tmAs, tmB0, tmB1;
   if (!make_map_u8(&tmA, g.aq, (uint64_t)g.P, (uint64_t)K)) return B200MOE_EDRIVER;
   if (!make_map_u8(&tmAs, g.aq, (uint64_t)g.P, (uint64_t)K, TC_AR)) return B200MOE_EDRIVER;
   if (!make_map_u8(&tmB0, g.w0, (uint64_t)g.E * g.I, (uint64_t)g.H)) return B200MOE_EDRIVER;
-  if (!make_map_u8(&tmB1, (GEMM2 || DENSE) ? g.w0 : g.w1, (uint64_t)g.E * g.I, (uint64_t)g.H)) return B200MOE_EDRIVER;
+  if (!make_map_u8(&tmB1, GATE_UP || (MODE == 4 && g.segs == 2) ? g.w1 : g.w0, (uint64_t)g.E * g.I, (uint64_t)g.H)) return B200MOE_EDRIVER;
   TcArgs a{};
   a.as_t = g.as_t;
   a.ld = g.ld;
   a.s0 = g.s0;
-  a.s1 = g.s1;
+  a.s1 = MODE == 4 && g.segs == 1 ? g.s0 : g.s1;
+  a.segs = g.segs;
+  a.dh = g.dh;
+  a.dwp = g.dwp;
+  a.g16 = g.g16;
   a.mtiles = g.mtiles;
   a.num_mtiles = g.num_mtiles;
   a.offsets = g.offsets;
@@ -870,9 +1040,12 @@ int launch_tc(const MoeGemmArgs& g, cudaStream_t st) {
     cudaFuncSetAttribute(moe_gemm_tc_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TC_SMEM_BYTES);
     cudaFuncSetAttribute(moe_gemm_tc_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TC_SMEM_BYTES);
     cudaFuncSetAttribute(moe_gemm_tc_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TC_SMEM_BYTES);
+    cudaFuncSetAttribute(moe_gemm_tc_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TC_SMEM_BYTES);
+    cudaFuncSetAttribute(moe_gemm_tc_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TC_SMEM_BYTES);
+    cudaFuncSetAttribute(moe_gemm_tc_kernel<5>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TC_SMEM_BYTES);
     di->attr_set = true;
   }
-  if (MODE != 0 && a.KS == 1 && !a.comb32 && !g.row_src && g.split.part) {
+  if (!GATE_UP && a.KS == 1 && !a.comb32 && !g.row_src && g.split.part) {
     const int64_t rows = g.P / (g.E < g.P ? g.E : g.P);  // of an average tile
     a.part = g.split.part;
     a.part_cnt = g.split.cnt;
@@ -918,3 +1091,6 @@ int moe_device_sm_count() { return device_sm_count(); }
 int moe_gemm1_tc(const MoeGemmArgs& a, cudaStream_t st) { return launch_tc<0>(a, st); }
 int moe_gemm2_tc(const MoeGemmArgs& a, cudaStream_t st) { return launch_tc<1>(a, st); }
 int moe_linear_tc(const MoeGemmArgs& a, cudaStream_t st) { return launch_tc<2>(a, st); }
+int moe_swiglu_grad_tc(const MoeGemmArgs& a, cudaStream_t st) { return launch_tc<3>(a, st); }
+int moe_dx_tc(const MoeGemmArgs& a, cudaStream_t st) { return launch_tc<4>(a, st); }
+int moe_dh_tc(const MoeGemmArgs& a, cudaStream_t st) { return launch_tc<5>(a, st); }

@@ -1,0 +1,797 @@
+// The gradients of the layer's entry points: routing, router product, weighted combine, experts, linear layer (formulas at
+// each declaration in include/b200moe.h).  The small kernels are here; the products are in gemm_tc.cu (FP8: dh, swiglu, dx)
+// and gemm_grad_tc.cu (bf16: weight gradients, the router's products).
+#include <algorithm>
+
+#include "internal.h"
+
+namespace {
+
+inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+struct Carve {  // offsets of a workspace's parts
+  size_t total = 0;
+  size_t take(size_t bytes) {
+    const size_t at = total;
+    total = align_up(total + bytes, 256);
+    return at;
+  }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// ---- routing ------------------------------------------------------------------------------------------------------
+// One warp per token; lane j holds slot j (k <= 32).  With p_j the score of slot j, S their sum and c the scale:
+//   renormalised    dp_j = c (dw_j - sum_i dw_i p_i / S) / S,   else   dp_j = c dw_j
+//   sigmoid         dl_e = p_e (1 - p_e) * (dp of the slots that chose e)
+//   softmax         dl_e = s_e * ((dp of the slots that chose e) - sum_i dp_i p_i)
+// Renormalised softmax weights depend on the selected logits alone (the last sum is zero): they are formed as a softmax
+// over those, so the row itself need not be read, and all other entries are exactly zero.
+struct RouteGradArgs {
+  float* dlogits;
+  const float* logits;
+  const float* logit_bias;
+  const int32_t* ids;
+  const void* dw;
+  int dw_dtype, E, k, score_func, renorm;
+  float scale;
+};
+constexpr int RT_WARPS = 4;
+template <bool VEC>  // rows are whole float4s
+__global__ void __launch_bounds__(RT_WARPS * 32)
+route_grad_kernel(const RouteGradArgs a, int64_t T) {
+  pdl_begin();
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * RT_WARPS + (threadIdx.x >> 5);
+  if (t >= T) return;
+  const float* row = a.logits + t * a.E;
+  const int E = a.E, k = a.k;
+  int id = lane < k ? a.ids[t * k + lane] : -1;
+  if (id >= E) id = -1;  // a dropped pair
+  const bool on = id >= 0;
+  const float dw = on ? moe_load_as_f32(a.dw, t * k + lane, a.dw_dtype) : 0.f;
+  const float l = on ? row[id] + (a.logit_bias ? a.logit_bias[id] : 0.f) : -INFINITY;
+  const bool softmax = a.score_func == B200MOE_SCORE_SOFTMAX;
+  float v = 0.f;       // what this slot adds to its expert's entry
+  float m = 0.f, inv = 0.f, c = 0.f;  // full softmax: dl_e = s_e * (... - c)
+  const bool dense = softmax && !a.renorm;
+  if (dense) {
+    m = -INFINITY;
+    for (int e = lane; e < E; e += 32) m = fmaxf(m, row[e] + (a.logit_bias ? a.logit_bias[e] : 0.f));
+    m = warp_max(m);
+    float sum = 0.f;
+    for (int e = lane; e < E; e += 32) sum += expf(row[e] + (a.logit_bias ? a.logit_bias[e] : 0.f) - m);
+    inv = 1.f / warp_sum(sum);
+    v = a.scale * dw;
+    c = warp_sum(on ? v * expf(l - m) * inv : 0.f);
+  } else if (softmax) {
+    m = warp_max(l);
+    const float p = on ? expf(l - m) : 0.f, w = p / warp_sum(p);
+    const float mean = warp_sum(on ? w * dw : 0.f);
+    v = on ? a.scale * w * (dw - mean) : 0.f;
+  } else {
+    const float p = 1.f / (1.f + expf(-l)), q = 1.f / (1.f + expf(l));  // q = 1 - p without its cancellation
+    if (a.renorm) {
+      const float S = warp_sum(on ? p : 0.f), w = p / S;
+      const float mean = warp_sum(on ? w * dw : 0.f);
+      v = on ? a.scale * w * q * (dw - mean) : 0.f;
+    } else {
+      v = on ? a.scale * dw * p * q : 0.f;
+    }
+  }
+  float* out = a.dlogits + t * E;
+  constexpr int V = VEC ? 4 : 1;
+  for (int base = 0; base < E; base += 32 * V) {  // (all lanes: the shuffles below need every slot's)
+    const int e0 = base + lane * V;
+    const bool in = e0 < E;
+    float add[V], o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) add[i] = 0.f, o[i] = dense && in ? row[e0 + i] : 0.f;
+    for (int j = 0; j < k; ++j) {  // (in slot order, should two slots name the same expert)
+      const int ej = __shfl_sync(0xffffffffu, id, j);
+      const float vj = __shfl_sync(0xffffffffu, v, j);
+#pragma unroll
+      for (int i = 0; i < V; ++i) add[i] += ej == e0 + i ? vj : 0.f;
+    }
+    if (!in) continue;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      o[i] = dense ? expf(o[i] + (a.logit_bias ? a.logit_bias[e0 + i] : 0.f) - m) * inv * (add[i] - c) : add[i];
+    if constexpr (VEC) *reinterpret_cast<float4*>(out + e0) = make_float4(o[0], o[1], o[2], o[3]);
+    else out[e0] = o[0];
+  }
+}
+
+// ---- weighted combine -----------------------------------------------------------------------------------------------
+// dy[t,j,:] = w[t,j] * dout[t,:], dw[t,j] = <dout[t,:], y[t,j,:]>: one block per token, dout's row in registers (up to
+// CG_COLS columns at a time), the token's rows of y through it.  Bound by HBM: k rows in, k rows out.
+constexpr int CG_THREADS = 256;
+constexpr int CG_VEC = 4;                            // 16-byte pieces of a row per thread
+constexpr int CG_COLS = CG_THREADS * 8 * CG_VEC;     // 8192
+constexpr int CG_MAXK = 32;
+__global__ void __launch_bounds__(CG_THREADS)
+combine_grad_kernel(__nv_bfloat16* dy, float* dw, const __nv_bfloat16* dout, const __nv_bfloat16* y, const void* w, int w_dtype,
+                    const int32_t* ids, int E, int k, int H) {
+  pdl_begin();
+  __shared__ float part[CG_THREADS / 32][CG_MAXK];
+  const int64_t t = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int c0 = 0; c0 < H; c0 += CG_COLS) {
+    uint4 d[CG_VEC];
+    int col[CG_VEC];
+#pragma unroll
+    for (int u = 0; u < CG_VEC; ++u) {
+      col[u] = c0 + (u * CG_THREADS + threadIdx.x) * 8;
+      d[u] = col[u] < H ? *reinterpret_cast<const uint4*>(dout + t * H + col[u]) : make_uint4(0, 0, 0, 0);
+    }
+    for (int j = 0; j < k; ++j) {
+      const int64_t p = t * k + j;
+      const bool on = !(ids && (ids[p] < 0 || ids[p] >= E));  // (a dropped slot: its row of y was never written)
+      const float wj = dy && on ? moe_load_as_f32(w, p, w_dtype) : 0.f;
+      uint4 yv[CG_VEC];
+#pragma unroll
+      for (int u = 0; u < CG_VEC; ++u)
+        yv[u] = dw && on && col[u] < H ? *reinterpret_cast<const uint4*>(y + p * H + col[u]) : make_uint4(0, 0, 0, 0);
+      float dot = 0.f;
+#pragma unroll
+      for (int u = 0; u < CG_VEC; ++u) {
+        if (col[u] >= H) continue;
+        const __nv_bfloat162 *d2 = reinterpret_cast<const __nv_bfloat162*>(&d[u]), *y2 = reinterpret_cast<const __nv_bfloat162*>(&yv[u]);
+        uint4 o;
+        __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 df = __bfloat1622float2(d2[i]), yf = __bfloat1622float2(y2[i]);
+          if (on) dot = fmaf(df.x, yf.x, fmaf(df.y, yf.y, dot));
+          o2[i] = on ? __floats2bfloat162_rn(wj * df.x, wj * df.y) : __floats2bfloat162_rn(0.f, 0.f);
+        }
+        if (dy) *reinterpret_cast<uint4*>(dy + p * H + col[u]) = o;
+      }
+      dot = warp_sum(dot);
+      if (lane == 0) part[warp][j] = (c0 ? part[warp][j] : 0.f) + dot;
+    }
+  }
+  __syncthreads();
+  if (dw && threadIdx.x < k) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < CG_THREADS / 32; ++i) s += part[i][threadIdx.x];
+    dw[t * k + threadIdx.x] = s;
+  }
+}
+
+// ---- operands of the experts' and the linear layer's products --------------------------------------------------------
+// Rows are read once: quantised (1 x 128, e4m3) and, where weight gradients are wanted, copied in bf16, both to the
+// positions of the row's slots (pos_of, -1 = dropped; NULL = row order).  A lane owns 16 consecutive columns, eight lanes
+// one 128-column group; a warp takes 512 columns of a row.  blockIdx.y: which of two tensors (tokens, gradients).
+struct PrepSide {
+  const __nv_bfloat16* src;  // [rows, H]
+  uint8_t* q;
+  float* s_t;                // [ceil(H/128), ld]
+  __nv_bfloat16* copy;       // NULL = no copy
+  int64_t rows;
+  int slots;                 // positions of a row: pos_of[row * slots + j]
+  float floor;
+};
+struct PrepArgs {
+  PrepSide side[2];
+  const int32_t* pos_of;
+  int64_t ld;
+  int H, warps_per_row;
+  float* acc32;              // fp32 [side 0's rows, H] cleared on the way, or NULL
+  MoeIdentityLists lists;    // written for side 0's rows (offsets NULL = none)
+};
+__global__ void __launch_bounds__(256)
+grad_prep_kernel(const PrepArgs a) {
+  pdl_begin();
+  const PrepSide& sd = a.side[blockIdx.y];
+  if (a.lists.offsets && blockIdx.x == 0 && blockIdx.y == 0) moe_write_identity_lists(a.lists, (int)sd.rows);
+  const int lane = threadIdx.x & 31;
+  const int64_t wi = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t r = wi / a.warps_per_row;
+  if (r >= sd.rows) return;  // uniform over the warp
+  const int H = a.H, c = (int)(wi - r * a.warps_per_row) * 512 + lane * 16;
+  const bool in = c < H;
+  uint4 raw[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) raw[i] = in ? *reinterpret_cast<const uint4*>(sd.src + r * H + c + i * 8) : make_uint4(0, 0, 0, 0);
+  if (a.acc32 && blockIdx.y == 0 && in) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(a.acc32 + r * H + c)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  float v[16], amax = 0.f;
+  const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(raw);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = __bfloat1622float2(b2[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  amax = fmaxf(amax, sd.floor);
+  const float inv = kFp8Max / amax, sc = amax / kFp8Max;
+  uint4 out;
+  out.x = moe_f32x4_to_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+  out.y = moe_f32x4_to_e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+  out.z = moe_f32x4_to_e4m3x4(v[8] * inv, v[9] * inv, v[10] * inv, v[11] * inv);
+  out.w = moe_f32x4_to_e4m3x4(v[12] * inv, v[13] * inv, v[14] * inv, v[15] * inv);
+  for (int j = 0; j < sd.slots; ++j) {
+    const int64_t p = a.pos_of ? a.pos_of[r * sd.slots + j] : r;
+    if (p < 0 || !in) continue;
+    *reinterpret_cast<uint4*>(sd.q + p * H + c) = out;
+    if ((lane & 7) == 0) sd.s_t[(int64_t)(c >> 7) * a.ld + p] = sc;
+    if (sd.copy) {
+      *reinterpret_cast<uint4*>(sd.copy + p * H + c) = raw[0];
+      *reinterpret_cast<uint4*>(sd.copy + p * H + c + 8) = raw[1];
+    }
+  }
+}
+int launch_prep(PrepArgs a, cudaStream_t st) {
+  a.warps_per_row = (a.H + 511) / 512;
+  const int64_t rows = std::max(a.side[0].rows, a.side[1].rows);
+  return moe_launch(grad_prep_kernel, dim3((unsigned)((rows * a.warps_per_row + 7) / 8), a.side[1].src ? 2 : 1), 256, 0, st, a);
+}
+
+// ---- last step of the experts' gradient ------------------------------------------------------------------------------
+// dx[t,:] = sum over the token's slots of y[t*k+j,:] (or acc32[t,:]) (+ add[t,:]), in slot order; dw[t,j] = the partial sums
+// of the slot's row, in column order (0 for a dropped slot)
+struct FinishArgs {
+  __nv_bfloat16* dx;  // NULL = not wanted
+  const __nv_bfloat16* y;
+  const float* acc32;
+  const __nv_bfloat16* add;
+  const int32_t* ids;
+  float* dw;          // NULL = not wanted
+  const float* dwp;
+  const int32_t *sorted, *pos_of;
+  int64_t T, ld, dx_blocks;
+  int E, k, H, parts;
+};
+__global__ void __launch_bounds__(256)
+grad_finish_kernel(const FinishArgs a) {
+  pdl_begin();
+  if (blockIdx.x >= a.dx_blocks) {
+    const int64_t r = ((int64_t)blockIdx.x - a.dx_blocks) * 256 + threadIdx.x, P = a.T * a.k;
+    if (r >= P) return;
+    if (a.pos_of[r] < 0) a.dw[r] = 0.f;
+    const int pair = a.sorted[r];
+    if (pair < 0) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < a.parts; ++i) s += a.dwp[(int64_t)i * a.ld + r];
+    a.dw[pair] = s;
+    return;
+  }
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int hv = a.H / 8;
+  if (idx >= a.T * hv) return;
+  const int64_t t = idx / hv;
+  const int c = (int)(idx - t * hv) * 8;
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+  auto add8 = [&](const uint4& raw) {
+    const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __bfloat1622float2(b2[i]);
+      acc[2 * i] += f.x, acc[2 * i + 1] += f.y;
+    }
+  };
+  if (a.acc32) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(a.acc32 + t * a.H + c + i * 4);
+      acc[4 * i] = v.x, acc[4 * i + 1] = v.y, acc[4 * i + 2] = v.z, acc[4 * i + 3] = v.w;
+    }
+  } else {
+    for (int j0 = 0; j0 < a.k; j0 += 4) {
+      uint4 raw[4];
+      bool on[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t p = t * a.k + j0 + u;
+        on[u] = j0 + u < a.k && a.ids[p] >= 0 && a.ids[p] < a.E;  // (a dropped slot has no row)
+        if (on[u]) raw[u] = *reinterpret_cast<const uint4*>(a.y + p * a.H + c);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (on[u]) add8(raw[u]);
+    }
+  }
+  if (a.add) add8(*reinterpret_cast<const uint4*>(a.add + t * a.H + c));
+  uint4 o;
+  __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o2[i] = __floats2bfloat162_rn(acc[2 * i], acc[2 * i + 1]);
+  *reinterpret_cast<uint4*>(a.dx + t * a.H + c) = o;
+}
+
+// ---- router product ----------------------------------------------------------------------------------------------------
+// dlogits as two bf16 numbers, v = hi + lo + (less than 2^-17 of v): the products run on the bf16 tensor cores and lose no
+// more than an fp32 sum does.  split [T, 2 Ep]: hi in columns [0, Ep), lo in [Ep, 2 Ep), Ep = E rounded up to a K step.
+// Four columns per thread.
+__global__ void __launch_bounds__(256)
+split_logits_kernel(__nv_bfloat16* split, const float* dlogits, int64_t T, int E, int Ep) {
+  pdl_begin();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = Ep / 4;
+  if (i >= T * per) return;
+  const int64_t t = i / per;
+  const int e0 = (int)(i - t * per) * 4;
+  __nv_bfloat16 hi[4], lo[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float v = e0 + u < E ? dlogits[t * E + e0 + u] : 0.f;
+    hi[u] = __float2bfloat16_rn(v);
+    const float rest = v - __bfloat162float(hi[u]);
+    lo[u] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.f);  // (an infinity is all in hi)
+  }
+  *reinterpret_cast<uint2*>(split + t * 2 * Ep + e0) = *reinterpret_cast<const uint2*>(hi);
+  *reinterpret_cast<uint2*>(split + t * 2 * Ep + Ep + e0) = *reinterpret_cast<const uint2*>(lo);
+}
+// dwr[e,h] (+)= sum over the parts, in order, of part[i][e,h] (hi) + part[i][Ep+e,h] (lo)
+__global__ void __launch_bounds__(256)
+router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int E, int Ep, int H) {
+  pdl_begin();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int hv = H / 4;
+  if (i >= (int64_t)E * hv) return;
+  const int64_t e = i / hv;
+  const int c = (int)(i - e * hv) * 4;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < parts; ++s) {
+    const float* p = part + ((int64_t)s * 2 * Ep + e) * H + c;
+    const float4 hi = *reinterpret_cast<const float4*>(p), lo = *reinterpret_cast<const float4*>(p + (int64_t)Ep * H);
+    acc[0] += hi.x + lo.x, acc[1] += hi.y + lo.y, acc[2] += hi.z + lo.z, acc[3] += hi.w + lo.w;
+  }
+  if (f32) {
+    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(dwr) + e * H + c);
+    float4 old = add ? *o : make_float4(0.f, 0.f, 0.f, 0.f);
+    *o = make_float4(old.x + acc[0], old.y + acc[1], old.z + acc[2], old.w + acc[3]);
+  } else {
+    __nv_bfloat162 o[2] = {__floats2bfloat162_rn(acc[0], acc[1]), __floats2bfloat162_rn(acc[2], acc[3])};
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(dwr) + e * H + c) = *reinterpret_cast<const uint2*>(o);
+  }
+}
+
+__global__ void grad_scales_kernel(float* __restrict__ dst, const __nv_bfloat16* a, const __nv_bfloat16* b, const __nv_bfloat16* c,
+                                   int64_t n) {  // block scales in fp32: dst = a | b | c (b, c may be NULL)
+  pdl_begin();
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) {
+    dst[i] = __bfloat162float(a[i]);
+    if (b) dst[n + i] = __bfloat162float(b[i]);
+    if (c) dst[2 * n + i] = __bfloat162float(c[i]);
+  }
+}
+
+// the gradient of weights that no row reached
+int zero_grad(void* p, size_t bytes, bool add, cudaStream_t st) {
+  if (!p || add) return B200MOE_OK;
+  const cudaError_t e = cudaMemsetAsync(p, 0, bytes, st);
+  return e == cudaSuccess ? B200MOE_OK : (int)e;
+}
+size_t grad_elem(int dtype) { return dtype == B200MOE_F32 ? 4 : 2; }
+bool grad_dtype_ok(int dtype, int accumulate) {
+  return (dtype == B200MOE_F32 && (accumulate == 0 || accumulate == 1)) || (dtype == B200MOE_BF16 && accumulate == 0);
+}
+
+}  // namespace
+
+extern "C" int b200moe_route_backward(float* dlogits, const float* logits, const float* logit_bias, const int32_t* ids,
+                                      const void* dw, int dw_dtype, int64_t T, int64_t E, int64_t k, int score_func, int renorm,
+                                      float scale, void* stream) {
+  MOE_CHECK_ARG(T >= 0 && E > 0 && k > 0);
+  MOE_CHECK_ARG(score_func == B200MOE_SCORE_SOFTMAX || score_func == B200MOE_SCORE_SIGMOID);
+  MOE_CHECK_ARG(dw_dtype == B200MOE_F32 || dw_dtype == B200MOE_BF16);
+  MOE_CHECK_SHAPE(E <= 1024 && k <= 32 && k <= E && T < (int64_t(1) << 31));
+  if (T == 0) return B200MOE_OK;
+  MOE_CHECK_ARG(dlogits && logits && ids && dw);
+  const RouteGradArgs a{dlogits, logits, logit_bias, ids, dw, dw_dtype, (int)E, (int)k, score_func, renorm, scale};
+  const unsigned grid = (unsigned)((T + RT_WARPS - 1) / RT_WARPS);
+  const bool vec = E % 4 == 0 && moe_aligned16(dlogits);
+  return moe_launch(vec ? route_grad_kernel<true> : route_grad_kernel<false>, grid, RT_WARPS * 32, 0, (cudaStream_t)stream, a, T);
+}
+
+extern "C" int b200moe_combine_backward(void* dy, float* dw, const void* dout, const void* y, const void* w, int w_dtype,
+                                        const int32_t* ids, int64_t E, int64_t T, int64_t k, int64_t H, void* stream) {
+  MOE_CHECK_ARG(T >= 0 && k > 0 && H > 0 && (!ids || E > 0));
+  MOE_CHECK_ARG(w_dtype == B200MOE_F32 || w_dtype == B200MOE_BF16 || w_dtype == B200MOE_F16);
+  MOE_CHECK_SHAPE(H % 8 == 0 && k <= CG_MAXK && T < (int64_t(1) << 31) && H < (int64_t(1) << 30));
+  if (T == 0) return B200MOE_OK;
+  MOE_CHECK_ARG((dy || dw) && dout && (!dy || w) && (!dw || y));
+  if ((dy && !moe_aligned16(dy)) || !moe_aligned16(dout) || (dw && !moe_aligned16(y))) return B200MOE_EALIGN;
+  return moe_launch(combine_grad_kernel, (unsigned)T, CG_THREADS, 0, (cudaStream_t)stream, reinterpret_cast<__nv_bfloat16*>(dy), dw,
+                    reinterpret_cast<const __nv_bfloat16*>(dout), reinterpret_cast<const __nv_bfloat16*>(y), w, w_dtype, ids, (int)E,
+                    (int)k, (int)H);
+}
+
+// ---- router product ---------------------------------------------------------------------------------------------------
+namespace {
+struct RouterLayout {
+  size_t split, part, total;
+  int Ep, parts;
+};
+RouterLayout router_layout(int64_t T, int64_t H, int64_t E) {
+  RouterLayout L{};
+  Carve w;
+  L.Ep = (int)align_up((size_t)E, 64);
+  // Few output tiles (E rows): the tokens are cut into parts, so that every SM has a tile; a part has 128 tokens at least.
+  // (By the part's sizes and not by the device that runs: a workspace fits wherever it was sized.)
+  const int64_t tiles = (2 * L.Ep / 128) * ((H + 255) / 256);
+  L.parts = (int)std::max<int64_t>(1, std::min<int64_t>(148 / tiles, T / 128));
+  L.split = w.take((size_t)T * 2 * L.Ep * 2);
+  L.part = w.take((size_t)L.parts * 2 * L.Ep * H * 4);
+  L.total = w.total;
+  return L;
+}
+}  // namespace
+
+extern "C" size_t b200moe_router_logits_backward_workspace_bytes(int64_t T, int64_t H, int64_t E) {
+  if (T < 0 || H <= 0 || E <= 0 || H % 8 || E > 1024 || T >= (1 << 24) || H >= (1 << 24)) return 0;
+  // (monotone in T: a smaller batch may be cut into fewer parts, never into more)
+  return router_layout(T, H, E).total;
+}
+
+extern "C" int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype, int accumulate, const float* dlogits, const void* x,
+                                              const void* wr, int64_t T, int64_t H, int64_t E, void* workspace,
+                                              size_t workspace_bytes, int32_t* status, void* stream) {
+  MOE_CHECK_ARG(T >= 0 && H > 0 && E > 0 && (dx || dwr));
+  MOE_CHECK_ARG(!dwr || grad_dtype_ok(dwr_dtype, accumulate));
+  MOE_CHECK_SHAPE(H % 8 == 0 && E <= 1024 && T < (1 << 24) && H < (1 << 24));
+  cudaStream_t st = (cudaStream_t)stream;
+  if (T == 0) return zero_grad(dwr, (size_t)E * H * grad_elem(dwr_dtype), accumulate, st);
+  MOE_CHECK_ARG(dlogits && (!dx || wr) && (!dwr || x));
+  if ((dx && !(moe_aligned16(dx) && moe_aligned16(wr))) || (dwr && !(moe_aligned16(dwr) && moe_aligned16(x)))) return B200MOE_EALIGN;
+  if (!moe_tc_available()) return B200MOE_EDRIVER;
+  const RouterLayout L = router_layout(T, H, E);
+  if (!workspace || workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return B200MOE_EWORKSPACE;
+  char* ws = reinterpret_cast<char*>(workspace);
+  __nv_bfloat16* split = reinterpret_cast<__nv_bfloat16*>(ws + L.split);
+  float* part = reinterpret_cast<float*>(ws + L.part);
+  int rc = moe_launch(split_logits_kernel, (unsigned)((T * (L.Ep / 4) + 255) / 256), 256, 0, st, split, dlogits, T, (int)E, L.Ep);
+  if (!rc && dwr) {
+    MoeWeightGradArgs g{};
+    g.a = split;
+    g.b0 = reinterpret_cast<const __nv_bfloat16*>(x);
+    g.out[0] = part;
+    g.P = T;
+    g.groups = L.parts, g.segs = 1, g.M = 2 * L.Ep, g.N = (int)H;
+    g.out_f32 = 1;
+    g.status = status;
+    rc = moe_weight_grad_tc(g, st);
+    if (!rc)
+      rc = moe_launch(router_dwr_kernel, (unsigned)((E * (H / 4) + 255) / 256), 256, 0, st, dwr, (int)(dwr_dtype == B200MOE_F32),
+                      accumulate, part, L.parts, (int)E, L.Ep, (int)H);
+  }
+  if (!rc && dx)
+    rc = moe_row_product_tc(reinterpret_cast<__nv_bfloat16*>(dx), split, reinterpret_cast<const __nv_bfloat16*>(wr), T, 2 * L.Ep, (int)E,
+                            L.Ep, (int)H, status, st);
+  return rc;
+}
+
+// ---- linear layer -----------------------------------------------------------------------------------------------------
+namespace {
+struct LinGradLayout {
+  size_t offsets, mtiles, nmt, q, s, sc32, part, cnt, y32, total;
+  int64_t ld;
+  int max_mtiles;
+};
+LinGradLayout lin_grad_layout(int64_t M, int64_t K, int64_t N, int scale_dtype) {
+  LinGradLayout L{};
+  Carve w;
+  const int64_t nN = (N + kBlock - 1) / kBlock;
+  L.ld = (int64_t)align_up((size_t)std::max<int64_t>(M, 1), kTileM);
+  L.max_mtiles = (int)(L.ld / kTileM);
+  L.offsets = w.take(2 * sizeof(int32_t));
+  L.mtiles = w.take((size_t)L.max_mtiles * 2 * sizeof(int32_t));
+  L.nmt = w.take(sizeof(int32_t));
+  L.q = w.take((size_t)L.ld * N);
+  L.s = w.take((size_t)nN * L.ld * sizeof(float));
+  L.sc32 = w.take(scale_dtype == B200MOE_BF16 ? (size_t)nN * (K / kBlock) * sizeof(float) : 0);
+  L.part = w.take(moe_split_part_bytes(M));
+  L.cnt = w.take(kSplitCounters * sizeof(int32_t));
+  L.total = w.total;
+  return L;
+}
+}  // namespace
+
+extern "C" size_t b200moe_linear_w8_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int scale_dtype) {
+  if (M < 0 || K <= 0 || N <= 0 || K % kBlock || N % 64 || M >= (1 << 24) || K >= (1 << 24) || N >= (1 << 24)) return 0;
+  return lin_grad_layout(M, K, N, scale_dtype).total;
+}
+
+extern "C" int b200moe_linear_w8_backward(void* dx, void* dw, int dw_dtype, int accumulate, const void* dy, const void* x,
+                                          const void* w, const void* scale, int scale_dtype, int64_t M, int64_t K, int64_t N,
+                                          void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  MOE_CHECK_ARG(M >= 0 && K > 0 && N > 0 && (dx || dw));
+  MOE_CHECK_ARG(!dw || grad_dtype_ok(dw_dtype, accumulate));
+  MOE_CHECK_ARG(scale_dtype == B200MOE_F32 || scale_dtype == B200MOE_BF16);
+  MOE_CHECK_SHAPE(K % kBlock == 0 && N % 64 == 0 && M < (1 << 24) && K < (1 << 24) && N < (1 << 24));
+  cudaStream_t st = (cudaStream_t)stream;
+  if (M == 0) return zero_grad(dw, (size_t)N * K * grad_elem(dw_dtype), accumulate, st);
+  MOE_CHECK_ARG(dy && (!dx || (w && scale)) && (!dw || x));
+  if (!moe_aligned16(dy) || (dx && !(moe_aligned16(dx) && moe_aligned16(w))) || (dw && !(moe_aligned16(dw) && moe_aligned16(x))))
+    return B200MOE_EALIGN;
+  if (!moe_tc_available()) return B200MOE_EDRIVER;
+  const LinGradLayout L = lin_grad_layout(M, K, N, scale_dtype);
+  if (!workspace || workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return B200MOE_EWORKSPACE;
+  char* ws = reinterpret_cast<char*>(workspace);
+  auto I32 = [&](size_t off) { return reinterpret_cast<int32_t*>(ws + off); };
+  int rc = B200MOE_OK;
+  if (dx) {
+    PrepArgs p{};
+    p.side[0] = PrepSide{reinterpret_cast<const __nv_bfloat16*>(dy), reinterpret_cast<uint8_t*>(ws + L.q),
+                         reinterpret_cast<float*>(ws + L.s), nullptr, M, 1, kGradAmaxFloor};
+    p.ld = L.ld;
+    p.H = (int)N;
+    p.lists = MoeIdentityLists{I32(L.offsets), I32(L.mtiles), I32(L.nmt), I32(L.cnt)};
+    rc = launch_prep(p, st);
+    if (rc) return rc;
+    const void* sc = scale;
+    if (scale_dtype == B200MOE_BF16) {
+      const int64_t n = ((N + kBlock - 1) / kBlock) * (K / kBlock);
+      float* sc32 = reinterpret_cast<float*>(ws + L.sc32);
+      rc = moe_launch(grad_scales_kernel, (unsigned)((n + 255) / 256), 256, 0, st, sc32, reinterpret_cast<const __nv_bfloat16*>(scale),
+                      nullptr, nullptr, n);
+      if (rc) return rc;
+      sc = sc32;
+    }
+    MoeGemmArgs g{};
+    g.aq = reinterpret_cast<const uint8_t*>(ws + L.q);
+    g.as_t = reinterpret_cast<const float*>(ws + L.s);
+    g.ld = L.ld;
+    g.div = 1;
+    g.w0 = reinterpret_cast<const uint8_t*>(w);
+    g.s0 = sc;
+    g.scale_dtype = B200MOE_F32;
+    g.mtiles = I32(L.mtiles);
+    g.num_mtiles = I32(L.nmt);
+    g.offsets = I32(L.offsets);
+    g.max_mtiles = L.max_mtiles;
+    g.P = M;
+    g.H = (int)K;
+    g.I = (int)N;
+    g.E = 1;
+    g.segs = 1;
+    g.split = MoeSplitBuffers{reinterpret_cast<float*>(ws + L.part), I32(L.cnt)};
+    g.out = reinterpret_cast<__nv_bfloat16*>(dx);
+    g.status = status;
+    rc = moe_dx_tc(g, st);
+    if (rc) return rc;
+  }
+  if (dw) {
+    MoeWeightGradArgs g{};
+    g.a = reinterpret_cast<const __nv_bfloat16*>(dy);
+    g.b0 = reinterpret_cast<const __nv_bfloat16*>(x);
+    g.out[0] = dw;
+    g.P = M;
+    g.groups = g.segs = 1, g.M = (int)N, g.N = (int)K;
+    g.out_f32 = dw_dtype == B200MOE_F32, g.add = accumulate;
+    g.status = status;
+    rc = moe_weight_grad_tc(g, st);
+  }
+  return rc;
+}
+
+// ---- experts ------------------------------------------------------------------------------------------------------------
+namespace {
+struct ExpGradLayout {
+  size_t offsets, sorted, pos_of, scratch, mtiles, nmt, cnt, xq, xs, dq, ds, dh, gq, gs, dwp, y, shared, sc32, x16, d16, g16, total;
+  int64_t P, ld;
+  int max_mtiles, ksplit;
+};
+ExpGradLayout exp_grad_layout(const b200moe_experts_backward_desc& d) {
+  ExpGradLayout L{};
+  Carve w;
+  const int64_t P = d.T * d.k, nH = d.H / kBlock, nI = d.I / kBlock;
+  L.P = P;
+  L.ld = (int64_t)align_up((size_t)P, kTileM);
+  L.max_mtiles = (int)(P / kTileM + std::min(d.E, P));  // (an expert with rows has less than one tile more than they fill)
+  L.ksplit = moe_choose_ksplit(P, d.E, d.H, 2 * d.I);
+  L.offsets = w.take((d.E + 1) * sizeof(int32_t));
+  L.sorted = w.take((size_t)P * sizeof(int32_t));
+  L.pos_of = w.take((size_t)P * sizeof(int32_t));
+  L.scratch = w.take(b200moe_permute_scratch_ints(P, d.E) * sizeof(int32_t));
+  L.mtiles = w.take((size_t)L.max_mtiles * 2 * sizeof(int32_t));
+  L.nmt = w.take(sizeof(int32_t));
+  L.cnt = w.take(kSplitCounters * sizeof(int32_t));
+  L.xq = w.take((size_t)P * d.H);
+  L.xs = w.take((size_t)nH * L.ld * sizeof(float));
+  L.dq = w.take((size_t)P * d.H);
+  L.ds = w.take((size_t)nH * L.ld * sizeof(float));
+  L.dh = w.take((size_t)L.max_mtiles * kTileM * d.I * sizeof(float));
+  L.gq = w.take((size_t)P * 2 * d.I);
+  L.gs = w.take((size_t)2 * nI * L.ld * sizeof(float));
+  L.dwp = w.take(d.per_slot ? 0 : (size_t)2 * nI * L.ld * sizeof(float));
+  L.y = w.take((size_t)P * d.H * 2);
+  // partial sums of shared tiles, or the fp32 rows that a split K range of dx adds into (small batches): never both in one launch
+  // (for min(P, limit) rows whatever P is, so that the workspace size never shrinks when T grows)
+  L.shared = w.take(std::max(moe_split_part_bytes(P), (size_t)std::min<int64_t>(P, 512) * d.H * sizeof(float)));
+  L.sc32 = w.take(d.scale_dtype == B200MOE_BF16 ? 3 * (size_t)d.E * nI * nH * sizeof(float) : 0);
+  if (d.weight_grads) {
+    L.x16 = w.take((size_t)P * d.H * 2);
+    L.d16 = w.take((size_t)P * d.H * 2);
+    L.g16 = w.take((size_t)P * 3 * d.I * 2);
+  }
+  L.total = w.total;
+  return L;
+}
+int check_exp_grad(const b200moe_experts_backward_desc* d) {
+  MOE_CHECK_ARG(d);
+  MOE_CHECK_ARG(d->T >= 0 && d->H > 0 && d->I > 0 && d->E > 0 && d->k > 0);
+  MOE_CHECK_ARG((d->per_slot == 0 || d->per_slot == 1) && (d->weight_grads == 0 || d->weight_grads == 1));
+  MOE_CHECK_ARG(d->scale_dtype == B200MOE_F32 || d->scale_dtype == B200MOE_BF16);
+  MOE_CHECK_ARG(d->w_dtype == B200MOE_F32 || d->w_dtype == B200MOE_BF16);
+  if (d->weight_grads) MOE_CHECK_ARG(grad_dtype_ok(d->grad_dtype, d->accumulate));
+  MOE_CHECK_SHAPE(d->H % kBlock == 0 && d->I % kBlock == 0);
+  MOE_CHECK_SHAPE(d->E <= 1024 && d->k < (1 << 24) && d->T < (1 << 24) && d->T * d->k < (1 << 24));
+  MOE_CHECK_SHAPE(d->H < (1 << 24) && d->I < (1 << 23) && d->E * d->I < (int64_t(1) << 31));
+  return B200MOE_OK;
+}
+}  // namespace
+
+extern "C" size_t b200moe_experts_backward_workspace_bytes(const b200moe_experts_backward_desc* d) {
+  if (check_exp_grad(d) != B200MOE_OK) return 0;
+  return exp_grad_layout(*d).total;
+}
+
+extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void* dw_up, void* dw_down, const void* dout,
+                                        const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* s_gate,
+                                        const void* s_up, const void* s_down, const int32_t* ids, const void* topk_w,
+                                        const void* add, const b200moe_experts_backward_desc* d, void* workspace,
+                                        size_t workspace_bytes, int32_t* status, void* stream) {
+  int rc = check_exp_grad(d);
+  if (rc) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool wgrad = d->weight_grads;
+  MOE_CHECK_ARG(dx || dw || wgrad);
+  if (wgrad) MOE_CHECK_ARG(dw_gate && dw_up && dw_down);
+  if (d->T == 0) {
+    if (wgrad)
+      for (void* p : {dw_gate, dw_up, dw_down}) {
+        rc = zero_grad(p, (size_t)d->E * d->I * d->H * grad_elem(d->grad_dtype), d->accumulate, st);
+        if (rc) return rc;
+      }
+    return B200MOE_OK;
+  }
+  MOE_CHECK_ARG(dout && x && w_gate && w_up && w_down && s_gate && s_up && s_down && ids);
+  MOE_CHECK_ARG(d->per_slot ? !topk_w && !dw : topk_w != nullptr);
+  MOE_CHECK_ARG(!add || dx);
+  for (const void* p : {(const void*)dx, dout, x, w_gate, w_up, w_down, add, (const void*)(wgrad ? dw_gate : nullptr),
+                        (const void*)(wgrad ? dw_up : nullptr), (const void*)(wgrad ? dw_down : nullptr)})
+    if (p && !moe_aligned16(p)) return B200MOE_EALIGN;
+  if (!moe_tc_available()) return B200MOE_EDRIVER;
+  const ExpGradLayout L = exp_grad_layout(*d);
+  if (!workspace || workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return B200MOE_EWORKSPACE;
+  char* ws = reinterpret_cast<char*>(workspace);
+  auto I32 = [&](size_t off) { return reinterpret_cast<int32_t*>(ws + off); };
+  auto F32 = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
+  auto U8 = [&](size_t off) { return reinterpret_cast<uint8_t*>(ws + off); };
+  auto B16 = [&](size_t off) { return reinterpret_cast<__nv_bfloat16*>(ws + off); };
+  const bool fused = L.ksplit > 1 && dx;  // dx's partial sums meet in fp32 rows
+
+  rc = moe_permute_impl(I32(L.sorted), I32(L.offsets), ids, d->T, d->k, d->E, I32(L.scratch), status, I32(L.pos_of), I32(L.mtiles),
+                        I32(L.nmt), L.max_mtiles, I32(L.cnt), stream);
+  if (rc) return rc;
+  const void *sg = s_gate, *su = s_up, *sd = s_down;
+  if (d->scale_dtype == B200MOE_BF16) {
+    const int64_t n = d->E * (d->I / kBlock) * (d->H / kBlock);
+    float* sc32 = F32(L.sc32);
+    rc = moe_launch(grad_scales_kernel, (unsigned)((n + 255) / 256), 256, 0, st, sc32, reinterpret_cast<const __nv_bfloat16*>(s_gate),
+                    reinterpret_cast<const __nv_bfloat16*>(s_up), reinterpret_cast<const __nv_bfloat16*>(s_down), n);
+    if (rc) return rc;
+    sg = sc32, su = sc32 + n, sd = sc32 + 2 * n;
+  }
+  PrepArgs p{};
+  p.side[0] = PrepSide{reinterpret_cast<const __nv_bfloat16*>(x), U8(L.xq), F32(L.xs), wgrad ? B16(L.x16) : nullptr, d->T, (int)d->k,
+                       kAmaxFloor};
+  p.side[1] = PrepSide{reinterpret_cast<const __nv_bfloat16*>(dout), U8(L.dq), F32(L.ds), wgrad ? B16(L.d16) : nullptr,
+                       d->per_slot ? L.P : d->T, d->per_slot ? 1 : (int)d->k, kGradAmaxFloor};
+  p.pos_of = I32(L.pos_of);
+  p.ld = L.ld;
+  p.H = (int)d->H;
+  p.acc32 = nullptr;
+  rc = launch_prep(p, st);
+  if (rc) return rc;
+
+  MoeGemmArgs g{};
+  g.aq = U8(L.dq);
+  g.as_t = F32(L.ds);
+  g.ld = L.ld;
+  g.row_map = I32(L.sorted);
+  g.div = (int)d->k;
+  g.w0 = reinterpret_cast<const uint8_t*>(w_down);
+  g.s0 = sd;
+  g.scale_dtype = B200MOE_F32;
+  g.mtiles = I32(L.mtiles);
+  g.num_mtiles = I32(L.nmt);
+  g.offsets = I32(L.offsets);
+  g.max_mtiles = L.max_mtiles;
+  g.P = L.P;
+  g.H = (int)d->H;
+  g.I = (int)d->I;
+  g.E = (int)d->E;
+  g.lists_ready = 1;  // the permutation's, with the preparation of the operands in between
+  g.split = MoeSplitBuffers{F32(L.shared), I32(L.cnt)};
+  g.dh = F32(L.dh);
+  g.status = status;
+  rc = moe_dh_tc(g, st);
+  if (rc) return rc;
+
+  MoeGemmArgs s = g;
+  s.aq = U8(L.xq);
+  s.as_t = F32(L.xs);
+  s.w0 = reinterpret_cast<const uint8_t*>(w_gate);
+  s.w1 = reinterpret_cast<const uint8_t*>(w_up);
+  s.s0 = sg;
+  s.s1 = su;
+  s.split = MoeSplitBuffers{};
+  s.hq = U8(L.gq);
+  s.hs_t = F32(L.gs);
+  s.comb_w = topk_w;
+  s.comb_wdt = d->w_dtype;
+  s.dwp = dw ? F32(L.dwp) : nullptr;
+  s.g16 = wgrad ? B16(L.g16) : nullptr;
+  rc = moe_swiglu_grad_tc(s, st);
+  if (rc) return rc;
+
+  float* acc32 = F32(L.shared);
+  if (dx) {
+    MoeGemmArgs y = s;
+    y.aq = s.hq;
+    y.as_t = s.hs_t;
+    y.segs = 2;
+    y.comb_w = nullptr;
+    y.split = g.split;
+    y.out = B16(L.y);
+    if (fused) {
+      const cudaError_t e = cudaMemsetAsync(acc32, 0, (size_t)d->T * d->H * sizeof(float), st);
+      if (e != cudaSuccess) return (int)e;
+      y.comb32 = acc32;
+      y.ksplit = L.ksplit;
+    }
+    rc = moe_dx_tc(y, st);
+    if (rc) return rc;
+  }
+  if (wgrad) {
+    MoeWeightGradArgs wg{};
+    wg.a = B16(L.g16);
+    wg.b0 = B16(L.x16);
+    wg.b1 = B16(L.d16);
+    wg.out[0] = dw_gate, wg.out[1] = dw_up, wg.out[2] = dw_down;
+    wg.offsets = I32(L.offsets);
+    wg.P = L.P;
+    wg.groups = (int)d->E, wg.segs = 3, wg.M = (int)d->I, wg.N = (int)d->H;
+    wg.out_f32 = d->grad_dtype == B200MOE_F32, wg.add = d->accumulate;
+    wg.status = status;
+    rc = moe_weight_grad_tc(wg, st);
+    if (rc) return rc;
+  }
+  if (dx || dw) {
+    FinishArgs f{};
+    f.dx = reinterpret_cast<__nv_bfloat16*>(dx);
+    f.y = B16(L.y);
+    f.acc32 = fused ? acc32 : nullptr;
+    f.add = reinterpret_cast<const __nv_bfloat16*>(add);
+    f.ids = ids;
+    f.dw = dw;
+    f.dwp = F32(L.dwp);
+    f.sorted = I32(L.sorted), f.pos_of = I32(L.pos_of);
+    f.T = d->T, f.ld = L.ld;
+    f.dx_blocks = dx ? (d->T * (d->H / 8) + 255) / 256 : 0;
+    f.E = (int)d->E, f.k = (int)d->k, f.H = (int)d->H, f.parts = (int)(d->I / 64);
+    rc = moe_launch(grad_finish_kernel, (unsigned)(f.dx_blocks + (dw ? (L.P + 255) / 256 : 0)), 256, 0, st, f);
+  }
+  return rc;
+}

@@ -57,6 +57,11 @@ struct MoeGemmArgs {
   // of that rank's buffer out_tbl[rank] (bf16 rows of H); overrides out/row_map
   const int32_t* row_src;
   const uint64_t* out_tbl;
+  // gradients (moe_dh_tc, moe_swiglu_grad_tc, moe_dx_tc)
+  int segs;                 // dx: weight tensors along K, w0 and with 2 also w1 (scales s0, s1)
+  float* dh;                // d in blocks of 128 x 128, [m-tile][I/128]: dh writes it, swiglu reads it
+  float* dwp;               // swiglu: partial sums of h * d, [I/64][ld], or NULL
+  __nv_bfloat16* g16;       // swiglu: bf16 rows [P, 3I] = dgate | dup | w * h, or NULL
   int hold_next;            // tensor-core kernels: the kernel behind this one starts after it and not beside it (see pdl_next)
   int lists_ready;          // mtiles / num_mtiles / offsets are older than the launch's direct predecessor (see pdl_wait)
   int32_t* status;
@@ -111,17 +116,42 @@ int moe_build_mtiles(int32_t* mtiles, int32_t* num_mtiles, const int32_t* offset
                      int max_mtiles, int32_t* split_cnt, cudaStream_t st);
 int moe_identity_lists(const MoeIdentityLists& lists, int64_t rows, cudaStream_t st);
 
+// K splits of a grouped product of P rows (K columns, H outputs each) on an MN-major weight operand
+int moe_choose_ksplit(int64_t P, int64_t E, int64_t H, int64_t K);
 int moe_gemm1_simple(const MoeGemmArgs& a, int act_mode, cudaStream_t st);
 int moe_gemm2_simple(const MoeGemmArgs& a, int act_mode, cudaStream_t st);
 int moe_gemm1_tc(const MoeGemmArgs& a, cudaStream_t st);
 int moe_gemm2_tc(const MoeGemmArgs& a, cudaStream_t st);
 // plain linear layer: out[r, :I] = A[r, :H] * w0^T, w0 [E*I, H] K-major with scales s0 [E, ceil(I/128), H/128]; bf16 rows of I
 int moe_linear_tc(const MoeGemmArgs& a, cudaStream_t st);
+// the products of the experts' gradients (gemm_tc.cu).  dh: d = A w0^T, A = aq [P,H], w0 = down; swiglu: A = aq [P,H], w0 = gate,
+// w1 = up, d -> hq [P, 2I] e4m3 = dgate | dup with scales hs_t [2I/128, ld]; the weight of row r is comb_w[row_map[r]] (NULL =
+// 1); dx: A = aq [P, segs * I], rows of H out as moe_gemm2_tc's
+int moe_dh_tc(const MoeGemmArgs& a, cudaStream_t st);
+int moe_swiglu_grad_tc(const MoeGemmArgs& a, cudaStream_t st);
+int moe_dx_tc(const MoeGemmArgs& a, cudaStream_t st);
 // the reference arithmetic (bf16 activations, weights dequantised to bf16) on the tensor cores; a16 = rows in sorted order
 int moe_gemm1_w8a16_tc(const MoeGemmArgs& a, cudaStream_t st);
 int moe_gemm2_w8a16_tc(const MoeGemmArgs& a, cudaStream_t st);
 int moe_gather_rows_bf16(__nv_bfloat16* dst, const __nv_bfloat16* x, const int32_t* row_map, int div, int64_t rows,
                          int H, cudaStream_t st);
+// weight gradients on the tensor cores (gemm_grad_tc.cu): out[seg][g * M + m, n] (+)= sum of a[r, seg * M + m] * b[r, n] over the
+// rows r of group g, b = b1 for segment 2, else b0.  Groups are [offsets[g], offsets[g+1]), clipped to P, or (offsets NULL) the
+// even parts of [0, P).  M % 128 == 0 unless there is one group and one segment; M, N % 8 == 0
+struct MoeWeightGradArgs {
+  const __nv_bfloat16* a;        // [P, segs * M]
+  const __nv_bfloat16 *b0, *b1;  // [P, N]
+  void* out[3];
+  const int32_t* offsets;
+  int64_t P;
+  int groups, segs, M, N;
+  int out_f32, add;              // add: to what `out` holds (fp32 only)
+  int32_t* status;
+};
+int moe_weight_grad_tc(const MoeWeightGradArgs& a, cudaStream_t st);
+// out[r, :N] = sum over k < K of a[r, k] * b[k % b_cycle, :N], b [b_rows, N] (rows past b_rows count as zeros); K, b_cycle % 64 == 0
+int moe_row_product_tc(__nv_bfloat16* out, const __nv_bfloat16* a, const __nv_bfloat16* b, int64_t rows, int K, int b_rows, int b_cycle,
+                       int N, int32_t* status, cudaStream_t st);
 int moe_f32_rows_to_bf16(__nv_bfloat16* out, const float* in, int64_t n, cudaStream_t st);
 int moe_device_sm_count();
 bool moe_tc_available();

@@ -28,6 +28,12 @@ class ExpertsDesc(Structure):
                 ("weights_bf16", c_int), ("stages", c_int), ("max_ctas", c_int)]
 
 
+class ExpertsBackwardDesc(Structure):
+    _fields_ = [("T", c_int64), ("H", c_int64), ("I", c_int64), ("E", c_int64), ("k", c_int64), ("per_slot", c_int),
+                ("scale_dtype", c_int), ("w_dtype", c_int), ("weight_grads", c_int), ("grad_dtype", c_int),
+                ("accumulate", c_int)]
+
+
 # name -> (restype, argtypes): every symbol include/b200moe.h declares
 SIGNATURES = {
     "b200moe_abi_version": (c_int, []),
@@ -71,6 +77,16 @@ SIGNATURES = {
     "b200moe_scaled_mm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "b200moe_scaled_mm": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+    "b200moe_route_backward": (c_int, [c_void_p] * 5 + [c_int, c_int64, c_int64, c_int64, c_int, c_int, c_float, c_void_p]),
+    "b200moe_router_logits_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "b200moe_router_logits_backward": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                               c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "b200moe_combine_backward": (c_int, [c_void_p] * 5 + [c_int, c_void_p] + [c_int64] * 4 + [c_void_p]),
+    "b200moe_linear_w8_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "b200moe_linear_w8_backward": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                           c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "b200moe_experts_backward_workspace_bytes": (c_size_t, [POINTER(ExpertsBackwardDesc)]),
+    "b200moe_experts_backward": (c_int, [c_void_p] * 16 + [POINTER(ExpertsBackwardDesc), c_void_p, c_size_t, c_void_p, c_void_p]),
     "b200moe_p2p_alloc": (c_int, [POINTER(c_void_p), c_size_t]),
     "b200moe_p2p_free": (c_int, [c_void_p]),
     "b200moe_p2p_export": (c_int, [c_char_p, c_void_p]),
