@@ -289,8 +289,8 @@ int b200moe_scaled_mm(void* out, int out_dtype, const void* a, const void* b, co
 int b200moe_route_backward(float* dlogits, const float* logits, const float* logit_bias, const int32_t* ids, const void* dw,
                            int dw_dtype, int64_t T, int64_t E, int64_t k, int score_func, int renorm, float scale, void* stream);
 
-/* Of b200moe_router_logits: dx[T,H] (bf16) = dlogits[T,E] . wr[E,H], dwr[E,H] = dlogits^T . x[T,H].  dlogits fp32 (taken
- * as two bf16 numbers each, 2^-17 relative); dx or dwr may be NULL, and then wr or x too.  H % 8 == 0, E <= 1024. */
+/* Of b200moe_router_logits: dx[T,H] (bf16) = dlogits[T,E] . wr[E,H], dwr[E,H] = dlogits^T . x[T,H].  dlogits fp32 (for dx
+ * taken to 2^-17 relative, for dwr in full); dx or dwr may be NULL, and then wr or x too.  H % 8 == 0, E <= 1024. */
 size_t b200moe_router_logits_backward_workspace_bytes(int64_t T, int64_t H, int64_t E);
 int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype, int accumulate, const float* dlogits, const void* x,
                                    const void* wr, int64_t T, int64_t H, int64_t E, void* workspace, size_t workspace_bytes,

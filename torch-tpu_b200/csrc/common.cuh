@@ -67,8 +67,8 @@ __device__ __forceinline__ void pdl_begin() {
   pdl_next();
 }
 template <typename... KArgs, typename... Args>
-inline int moe_launch_as(bool overlap, int cluster_y, void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem,
-                         cudaStream_t st, Args&&... args) {
+inline int moe_launch_clusters(bool overlap, dim3 cluster, void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem,
+                               cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
@@ -78,16 +78,20 @@ inline int moe_launch_as(bool overlap, int cluster_y, void (*kernel)(KArgs...), 
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = overlap ? 1 : 0;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = at[1].val.clusterDim.z = 1;
-  at[1].val.clusterDim.y = (unsigned)cluster_y;
+  at[1].val.clusterDim.x = cluster.x, at[1].val.clusterDim.y = cluster.y, at[1].val.clusterDim.z = cluster.z;
   cfg.attrs = at;
-  cfg.numAttrs = cluster_y > 1 ? 2 : 1;
+  cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return (int)e;
   }
   return B200MOE_OK;
+}
+template <typename... KArgs, typename... Args>
+inline int moe_launch_as(bool overlap, int cluster_y, void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem,
+                         cudaStream_t st, Args&&... args) {
+  return moe_launch_clusters(overlap, dim3(1, (unsigned)cluster_y, 1), kernel, grid, block, smem, st, static_cast<Args&&>(args)...);
 }
 template <typename... KArgs, typename... Args>
 inline int moe_launch(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args) {

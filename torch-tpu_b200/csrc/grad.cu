@@ -317,8 +317,9 @@ grad_finish_kernel(const FinishArgs a) {
 }
 
 // ---- router product ----------------------------------------------------------------------------------------------------
-// dlogits as two bf16 numbers, v = hi + lo + (less than 2^-17 of v): the products run on the bf16 tensor cores and lose no
-// more than an fp32 sum does.  split [T, 2 Ep]: hi in columns [0, Ep), lo in [Ep, 2 Ep), Ep = E rounded up to a K step.
+// dlogits as three bf16 numbers whose sum is the fp32 value (8 bits each; two leave 2.4e-6 of a result's norm behind): the
+// products run on the bf16 tensor cores and lose no more than an fp32 product does.  split [T, 3 Ep], Ep = E rounded up to a
+// K step: dx, which is rounded to bf16, takes the first two as a K range of 2 Ep; dwr takes all three as 3 Ep rows of output.
 // Four columns per thread.
 __global__ void __launch_bounds__(256)
 split_logits_kernel(__nv_bfloat16* split, const float* dlogits, int64_t T, int E, int Ep) {
@@ -328,18 +329,23 @@ split_logits_kernel(__nv_bfloat16* split, const float* dlogits, int64_t T, int E
   if (i >= T * per) return;
   const int64_t t = i / per;
   const int e0 = (int)(i - t * per) * 4;
-  __nv_bfloat16 hi[4], lo[4];
+  __nv_bfloat162 o[3][2];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const float v = e0 + u < E ? dlogits[t * E + e0 + u] : 0.f;
-    hi[u] = __float2bfloat16_rn(v);
-    const float rest = v - __bfloat162float(hi[u]);
-    lo[u] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.f);  // (an infinity is all in hi)
+    float v = e0 + u < E ? dlogits[t * E + e0 + u] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const __nv_bfloat16 b = __float2bfloat16_rn(v);
+      if (u & 1) o[i][u >> 1].y = b;
+      else o[i][u >> 1].x = b;
+      const float rest = v - __bfloat162float(b);
+      v = isfinite(rest) ? rest : 0.f;  // (an infinity is all in the first)
+    }
   }
-  *reinterpret_cast<uint2*>(split + t * 2 * Ep + e0) = *reinterpret_cast<const uint2*>(hi);
-  *reinterpret_cast<uint2*>(split + t * 2 * Ep + Ep + e0) = *reinterpret_cast<const uint2*>(lo);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(split + (t * 3 + i) * Ep + e0) = *reinterpret_cast<const uint2*>(o[i]);
 }
-// dwr[e,h] (+)= sum over the parts, in order, of part[i][e,h] (hi) + part[i][Ep+e,h] (lo)
+// dwr[e,h] (+)= sum over the parts, in order, of part[i][e,h] + (part[i][Ep+e,h] + part[i][2Ep+e,h])
 __global__ void __launch_bounds__(256)
 router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int E, int Ep, int H) {
   pdl_begin();
@@ -350,9 +356,10 @@ router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int
   const int c = (int)(i - e * hv) * 4;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < parts; ++s) {
-    const float* p = part + ((int64_t)s * 2 * Ep + e) * H + c;
-    const float4 hi = *reinterpret_cast<const float4*>(p), lo = *reinterpret_cast<const float4*>(p + (int64_t)Ep * H);
-    acc[0] += hi.x + lo.x, acc[1] += hi.y + lo.y, acc[2] += hi.z + lo.z, acc[3] += hi.w + lo.w;
+    const float* p = part + ((int64_t)s * 3 * Ep + e) * H + c;
+    const float4 v0 = *reinterpret_cast<const float4*>(p), v1 = *reinterpret_cast<const float4*>(p + (int64_t)Ep * H),
+                 v2 = *reinterpret_cast<const float4*>(p + (int64_t)2 * Ep * H);
+    acc[0] += v0.x + (v1.x + v2.x), acc[1] += v0.y + (v1.y + v2.y), acc[2] += v0.z + (v1.z + v2.z), acc[3] += v0.w + (v1.w + v2.w);
   }
   if (f32) {
     float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(dwr) + e * H + c);
@@ -426,12 +433,18 @@ RouterLayout router_layout(int64_t T, int64_t H, int64_t E) {
   RouterLayout L{};
   Carve w;
   L.Ep = (int)align_up((size_t)E, 64);
-  // Few output tiles (E rows): the tokens are cut into parts, so that every SM has a tile; a part has 128 tokens at least.
-  // (By the part's sizes and not by the device that runs: a workspace fits wherever it was sized.)
-  const int64_t tiles = (2 * L.Ep / 128) * ((H + 255) / 256);
-  L.parts = (int)std::max<int64_t>(1, std::min<int64_t>(148 / tiles, T / 128));
-  L.split = w.take((size_t)T * 2 * L.Ep * 2);
-  L.part = w.take((size_t)L.parts * 2 * L.Ep * H * 4);
+  // A tile is 256 x 256 outputs and 74 CTA pairs work at a time.  The tokens are cut into parts so that the rounds of
+  // (tile, part) items come out short: K steps of an item, plus four for what an item costs at its end and in the sum of the parts.
+  // (The sizes alone decide, not the device: a workspace fits wherever it was sized.)
+  const int64_t tiles = (3 * L.Ep + 255) / 256 * ((H + 255) / 256), steps = (T + 63) / 64;
+  int64_t best = 0;
+  L.parts = 1;
+  for (int64_t p = 1; p <= 16 && p * 2 <= std::max<int64_t>(steps, 2); ++p) {
+    const int64_t cost = (tiles * p + 73) / 74 * ((steps + p - 1) / p + 4);
+    if (p == 1 || cost < best) best = cost, L.parts = (int)p;
+  }
+  L.split = w.take((size_t)T * 3 * L.Ep * 2);
+  L.part = w.take((size_t)std::min<int64_t>(16, std::max<int64_t>(steps / 2, 1)) * 3 * L.Ep * H * 4);  // (for any number of parts: never smaller for more tokens)
   L.total = w.total;
   return L;
 }
@@ -439,7 +452,6 @@ RouterLayout router_layout(int64_t T, int64_t H, int64_t E) {
 
 extern "C" size_t b200moe_router_logits_backward_workspace_bytes(int64_t T, int64_t H, int64_t E) {
   if (T < 0 || H <= 0 || E <= 0 || H % 8 || E > 1024 || T >= (1 << 24) || H >= (1 << 24)) return 0;
-  // (monotone in T: a smaller batch may be cut into fewer parts, never into more)
   return router_layout(T, H, E).total;
 }
 
@@ -466,7 +478,7 @@ extern "C" int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype
     g.b0 = reinterpret_cast<const __nv_bfloat16*>(x);
     g.out[0] = part;
     g.P = T;
-    g.groups = L.parts, g.segs = 1, g.M = 2 * L.Ep, g.N = (int)H;
+    g.groups = L.parts, g.segs = 1, g.M = 3 * L.Ep, g.N = (int)H;
     g.out_f32 = 1;
     g.status = status;
     rc = moe_weight_grad_tc(g, st);
@@ -475,8 +487,8 @@ extern "C" int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype
                       accumulate, part, L.parts, (int)E, L.Ep, (int)H);
   }
   if (!rc && dx)
-    rc = moe_row_product_tc(reinterpret_cast<__nv_bfloat16*>(dx), split, reinterpret_cast<const __nv_bfloat16*>(wr), T, 2 * L.Ep, (int)E,
-                            L.Ep, (int)H, status, st);
+    rc = moe_row_product_tc(reinterpret_cast<__nv_bfloat16*>(dx), split, 3 * L.Ep, reinterpret_cast<const __nv_bfloat16*>(wr), T,
+                            2 * L.Ep, (int)E, L.Ep, (int)H, status, st);
   return rc;
 }
 

@@ -137,7 +137,7 @@ int moe_gather_rows_bf16(__nv_bfloat16* dst, const __nv_bfloat16* x, const int32
                          int H, cudaStream_t st);
 // weight gradients on the tensor cores (gemm_grad_tc.cu): out[seg][g * M + m, n] (+)= sum of a[r, seg * M + m] * b[r, n] over the
 // rows r of group g, b = b1 for segment 2, else b0.  Groups are [offsets[g], offsets[g+1]), clipped to P, or (offsets NULL) the
-// even parts of [0, P).  M % 128 == 0 unless there is one group and one segment; M, N % 8 == 0
+// even parts of [0, P).  M % 32 == 0, with several segments M % 128 == 0; N % 8 == 0
 struct MoeWeightGradArgs {
   const __nv_bfloat16* a;        // [P, segs * M]
   const __nv_bfloat16 *b0, *b1;  // [P, N]
@@ -149,9 +149,9 @@ struct MoeWeightGradArgs {
   int32_t* status;
 };
 int moe_weight_grad_tc(const MoeWeightGradArgs& a, cudaStream_t st);
-// out[r, :N] = sum over k < K of a[r, k] * b[k % b_cycle, :N], b [b_rows, N] (rows past b_rows count as zeros); K, b_cycle % 64 == 0
-int moe_row_product_tc(__nv_bfloat16* out, const __nv_bfloat16* a, const __nv_bfloat16* b, int64_t rows, int K, int b_rows, int b_cycle,
-                       int N, int32_t* status, cudaStream_t st);
+// out[r, :N] = sum over k < K of a[r * lda + k] * b[k % b_cycle, :N], b [b_rows, N] (rows past b_rows count as zeros); K, b_cycle % 64 == 0
+int moe_row_product_tc(__nv_bfloat16* out, const __nv_bfloat16* a, int lda, const __nv_bfloat16* b, int64_t rows, int K, int b_rows,
+                       int b_cycle, int N, int32_t* status, cudaStream_t st);
 int moe_f32_rows_to_bf16(__nv_bfloat16* out, const float* in, int64_t n, cudaStream_t st);
 int moe_device_sm_count();
 bool moe_tc_available();
