@@ -10,13 +10,13 @@
 // columns, the leader issues MMAs of M256 N256 K16 that read both CTAs' shared memory, each CTA's tensor memory receives
 // its 128 rows.  One CTA alone moves 48 KB into shared memory and as much out of it per 512-cycle K step (M128 N256 K64), which
 // is more than the 128 bytes per cycle that shared memory has; a pair moves 32 KB per CTA.
-// 12 warps per CTA: warp 0 = TMA producer, warp 1 = MMA issuer (leader) and tails, warps 4..11 = epilogue (lane quarter =
+// 12 warps per CTA: warp 0 = TMA producer, warp 1 = MMA issuer (leader) and TMEM owner, warp 2 = tails, warps 4..11 = epilogue (lane quarter =
 // warp % 4, column half = (warp - 4) / 4).  Five stages of 32 KB; two accumulators of 256 TMEM columns, so that the epilogue
 // of a tile runs beside the next tile's MMAs.  Results leave through swizzled shared-memory patches by TMA stores (or fp32
 // reductions), 32 rows x 128 bytes at a time.
 //
 // A group's last K step may reach past its end, into the next group's rows (or rows that nobody wrote).  MMAs are 16 rows
-// deep, so only rows up to the next multiple of 16 matter: where there are any, each CTA's warp 1 overwrites them in its
+// deep, so only rows up to the next multiple of 16 matter: where there are any, each CTA's warp 2 overwrites them in its
 // operands with zeros before the leader may use the stage - in the MN-major layout row r of a box is the 128 bytes at r * 128,
 // so the tail is one contiguous run per box.  (Rows past the end of the whole tensor are zeros already: TMA fills them.)
 //
@@ -34,7 +34,12 @@ namespace {
 
 constexpr int GG_EPI_WARPS = 8;
 constexpr int GG_THREADS = 128 + 32 * GG_EPI_WARPS;
-constexpr int GG_STAGES = 5;
+#ifndef GGS
+#define GGS 5
+#define GGP 2
+#endif
+constexpr int GG_STAGES = GGS;
+constexpr int GG_PATCHES = GGP;
 constexpr int GG_BK = 64;
 constexpr int GG_BOX_BYTES = GG_BK * 128;          // an MN-major box: 64 rows of K x 128 bytes
 constexpr int GG_A_BYTES = 128 * GG_BK * 2;        // 16 KB: this CTA's 128 of the tile's 256 rows (M)
@@ -58,7 +63,7 @@ struct GgShared {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr size_t GG_SMEM_BYTES = 1024 + (size_t)GG_STAGES * GG_STAGE_BYTES + 2 * GG_EPI_WARPS * GG_PATCH_BYTES + sizeof(GgShared);
+constexpr size_t GG_SMEM_BYTES = 1024 + (size_t)GG_STAGES * GG_STAGE_BYTES + GG_PATCHES * GG_EPI_WARPS * GG_PATCH_BYTES + sizeof(GgShared);
 static_assert(GG_SMEM_BYTES <= 232448, "more than the 227 KB of shared memory a CTA can have");
 
 struct GgArgs {
@@ -135,7 +140,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* patches = smem + (size_t)GG_STAGES * GG_STAGE_BYTES;
-  GgShared* sh = reinterpret_cast<GgShared*>(patches + 2 * GG_EPI_WARPS * GG_PATCH_BYTES);
+  GgShared* sh = reinterpret_cast<GgShared*>(patches + GG_PATCHES * GG_EPI_WARPS * GG_PATCH_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = blockIdx.x & 1;  // a pair is two neighbouring blocks of the grid (CTA pairs lie along x)
   const int pair0 = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -170,7 +175,12 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   const int per_group = a.segs * a.MT * a.NT, items = a.groups * per_group;
   struct Item {
-    int g, seg, mt, nt, beg, end;  // K range [beg, end)
+    int g, seg, mt, nt, beg, end;  // K range [beg, end); `end` is clipped to P by fixed(), when the value is needed and not
+                                   // when it is loaded: every role asks for its next item's range one item ahead
+  };
+  auto fixed = [&](Item w) {
+    if (!ROWS) w.end = min(w.end, a.P);
+    return w;
   };
   // n-tile fastest: the pairs that run together share a few m-tiles' columns of A and read all of B's
   auto item_of = [&](int t) {
@@ -185,11 +195,11 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       w.beg = 0, w.end = a.K;
     } else if (a.offsets) {
       w.beg = a.offsets[w.g];
-      w.end = min(a.offsets[w.g + 1], a.P);
+      w.end = a.offsets[w.g + 1];
     } else {  // whole K steps to each part
       const int64_t steps = (a.P + GG_BK - 1) / GG_BK;
       w.beg = (int)(steps * w.g / a.groups) * GG_BK;
-      w.end = min((int)(steps * (w.g + 1) / a.groups) * GG_BK, a.P);
+      w.end = (int)(steps * (w.g + 1) / a.groups) * GG_BK;
     }
     return w;
   };
@@ -209,7 +219,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       Item nx{};
       if (pair0 < items) nx = item_of(pair0);
       for (int t = pair0; t < items && ok; t += pairs) {
-        const Item w = nx;
+        const Item w = fixed(nx);
         if (t + pairs < items) nx = item_of(t + pairs);  // its row range is on the way while this item loads
         const CUtensorMap* tmB = w.seg == 2 ? &tmB1 : &tmB0;
         const int m0 = w.mt * 256 + rank * 128, n0 = w.nt * 256 + rank * 128;
@@ -239,40 +249,19 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer (leader) and tails (both CTAs)
+  } else if (warp == 1 && leader) {
+    // ------------------------------------------------------------------ MMA issuer (one thread; the warp stays together)
     const uint32_t idesc = gg_idesc(ROWS ? 0 : 1);
     const uint64_t adesc0 = ROWS ? make_smem_desc(smem_base, 16, 1024) : make_smem_desc(smem_base, GG_BOX_BYTES, 1024);
     const uint64_t bdesc0 = make_smem_desc(smem_base + GG_A_BYTES, GG_BOX_BYTES, 1024);
-    uint32_t s = 0, ph = 0, n = 0, tail_ph = 0;
+    uint32_t s = 0, ph = 0, n = 0;
     bool ok = true;
-    // the rows behind the group's last one, up to the next multiple of 16, count as zeros
-    auto clear_tail = [&](int rows) {
-      if (!gg_wait(smem_u32(&sh->tail[0]) + s * 8, (tail_ph >> s) & 1, abort_flag)) return false;
-      tail_ph ^= 1u << s;
-      const int from = rows * 8, each = ((rows + 15) & ~15) * 8 - from;  // in 16-byte units of a box
-      uint4* box = reinterpret_cast<uint4*>(smem + (size_t)s * GG_STAGE_BYTES);
-      for (int i = lane; i < 4 * each; i += 32) box[(i / each) * (GG_BOX_BYTES / 16) + from + i % each] = make_uint4(0, 0, 0, 0);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) gg_arrive(gg_in_cta(smem_u32(&sh->full[0]) + s * 8, 0));
-      return true;
-    };
     Item nx{};
     if (pair0 < items) nx = item_of(pair0);
     for (int t = pair0; t < items && ok; t += pairs) {
-      const Item w = nx;
+      const Item w = fixed(nx);
       if (t + pairs < items) nx = item_of(t + pairs);
-      const int tail = tail_rows(w);
-      if (!leader) {
-        const int steps = (max(w.end - w.beg, 0) + GG_BK - 1) / GG_BK;
-        if (steps > 0) {
-          s = (s + steps - 1) % GG_STAGES;
-          if (tail) ok = clear_tail(tail);
-          s = (s + 1) % GG_STAGES;
-        }
-        continue;
-      }
+      const bool tail = tail_rows(w) != 0;
       const int step = piece(w);
       for (int beg = w.beg; beg < w.end && ok; beg += step, ++n) {
         const int end = min(beg + step, w.end);
@@ -282,15 +271,12 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           break;
         }
         for (int r = beg; r < end; r += GG_BK) {
-          if (tail && w.end - r < GG_BK && !clear_tail(tail)) {
-            ok = false;
-            break;
-          }
           if (!gg_wait(smem_u32(&sh->full[0]) + s * 8, ph, abort_flag)) {
             ok = false;
             break;
           }
-          // (the other CTA's zeros were written by its threads: theirs to see takes more than what a copy's arrival gives)
+          // (zeros behind the group's end were written by threads, of the other CTA too: to see theirs takes more than what a
+          // copy's arrival gives)
           if (tail && w.end - r < GG_BK) asm volatile("fence.acq_rel.cluster;" ::: "memory");
           if (lane == 0) {
             tc_fence_after();
@@ -308,20 +294,45 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         __syncwarp();
       }
     }
+  } else if (warp == 2 && !ROWS) {
+    // ------------------------------------------------------------------ tails (both CTAs)
+    // the rows behind a group's last one, up to the next multiple of 16, become zeros as soon as the step's copies have landed
+    uint32_t at = 0, tail_ph = 0;  // K steps before the item; one phase bit per stage
+    Item nx{};
+    if (pair0 < items) nx = item_of(pair0);
+    for (int t = pair0; t < items; t += pairs) {
+      const Item w = fixed(nx);
+      if (t + pairs < items) nx = item_of(t + pairs);
+      at += (uint32_t)(max(w.end - w.beg, 0) + GG_BK - 1) / GG_BK;
+      const int rows = w.beg < w.end ? tail_rows(w) : 0;
+      if (!rows) continue;
+      const uint32_t s = (at - 1) % GG_STAGES;
+      if (!gg_wait(smem_u32(&sh->tail[0]) + s * 8, (tail_ph >> s) & 1, abort_flag)) break;
+      tail_ph ^= 1u << s;
+      uint4* box = reinterpret_cast<uint4*>(smem + (size_t)s * GG_STAGE_BYTES);
+      const int end = ((rows + 15) & ~15) * 8;  // in 16-byte units of a box
+      for (int i = rows * 8 + lane; i < end; i += 32) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) box[b * (GG_BOX_BYTES / 16) + i] = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) gg_arrive(gg_in_cta(smem_u32(&sh->full[0]) + s * 8, 0));
+    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue
     if (F32) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(GG_REG_HI));
     const int q = warp & 3, cg = (warp - 4) >> 2;
-    uint8_t* const patch0 = patches + (warp - 4) * (2 * GG_PATCH_BYTES);
+    uint8_t* const patch0 = patches + (warp - 4) * (GG_PATCHES * GG_PATCH_BYTES);
     const uint32_t tmem_empty_leader = gg_in_cta(smem_u32(&sh->tmem_empty[0]), 0);
     uint32_t n = 0;
     int stores = 0;
     bool ok = true;
     // the patch that the next store takes, once the store before the last has read it
     auto next_patch = [&]() {
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(GG_PATCHES - 1) : "memory");
       __syncwarp();
-      return reinterpret_cast<uint4*>(patch0 + (stores & 1) * GG_PATCH_BYTES);
+      return reinterpret_cast<uint4*>(patch0 + (stores % GG_PATCHES) * GG_PATCH_BYTES);
     };
     auto send_patch = [&](const CUtensorMap* map, const uint4* patch, int c0, int c1, bool add) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -333,8 +344,11 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       ++stores;
     };
     constexpr int PER = F32 ? 32 : 64;  // columns of a patch
+    Item nx{};
+    if (pair0 < items) nx = item_of(pair0);
     for (int t = pair0; t < items && ok; t += pairs) {
-      const Item w = item_of(t);
+      const Item w = fixed(nx);
+      if (t + pairs < items) nx = item_of(t + pairs);
       const CUtensorMap* map = w.seg == 0 ? &tmC0 : w.seg == 1 ? &tmC1 : &tmC2;
       const int mrow = w.mt * 256 + rank * 128 + q * 32, row = w.g * a.out_rows + mrow, col0 = w.nt * 256 + cg * 128;
       const bool rows_here = mrow < a.M;

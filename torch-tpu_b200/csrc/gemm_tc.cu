@@ -381,6 +381,10 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (row < row_end) dst[i] = a.row_src ? a.row_src[row] : a.row_map ? a.row_map[row] : row;
         }
       }
+      if (MODE == 3 && lane == 0)  // the item's block of d on its way to L2: its epilogue waits for it with nothing else to do
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<const float4*>(a.dh) + dh_index(w.mt, nI, w.nt, 0, 0, 0, 0)),
+                     "r"((min(row_end - row0, 128) + 31) / 32 * 16384)
+                     : "memory");
       float wv = 0.f;  // lanes 0..3: S0[w0i], S1[w1i], S0[w0i + sstep], S1[w1i + sstep]
       if (lane < 2 || (lane < 4 && w.KB > 1)) wv = scales_of(lane & 1, w.kb0 + (lane >> 1))[((lane & 1) ? w1i : w0i) + ((lane >> 1) ? sstep : 0)];
       // the slot is free once every epilogue warp has taken item n - 1 out of it
@@ -679,19 +683,24 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         float amax_u = 0.f, dot = 0.f;
         const float4* dsrc = reinterpret_cast<const float4*>(a.dh);
         if (warp_has_rows && ok) {
+          // 16 columns at a time; the next sixteen's d is on the way meanwhile
+          float4 dv[2][4];
+          auto load_d = [&](int c16, float4 (&v)[4]) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {  // 32 columns each
-            float4 dv[8];
+            for (int i = 0; i < 4; ++i)
+              v[i] = valid ? __ldcg(dsrc + dh_index(w.mt, nI3, nt, q, cg, c16 * 4 + i, lane)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          };
+          load_d(0, dv[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dv[i] = valid ? __ldcg(dsrc + dh_index(w.mt, nI3, nt, q, cg, half * 8 + i, lane)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c16 = 0; c16 < 4; ++c16) {
+            if (c16 < 3) load_d(c16 + 1, dv[(c16 + 1) & 1]);
 #pragma unroll
-            for (int v4 = 0; v4 < 4; ++v4) {
+            for (int v4 = 0; v4 < 2; ++v4) {
               uint32_t ow[4];
 #pragma unroll
               for (int w4 = 0; w4 < 4; ++w4) {
-                const int i = half * 16 + v4 * 4 + w4;  // pair of columns
-                const float4 d4 = dv[v4 * 2 + (w4 >> 1)];
+                const int i = c16 * 8 + v4 * 4 + w4;  // pair of columns
+                const float4 d4 = dv[c16 & 1][v4 * 2 + (w4 >> 1)];
                 const float2 g = unpack2(acc[0][i]), u = unpack2(acc[1][i]);
                 const float d[2] = {(w4 & 1) ? d4.z : d4.x, (w4 & 1) ? d4.w : d4.y}, gg[2] = {g.x, g.y}, uu[2] = {u.x, u.y};
                 float dg[2], du[2], hw[2];
@@ -710,9 +719,9 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 amax_u = fmaxf(amax_u, fmaxf(fabsf(du[0]), fabsf(du[1])));
                 ow[w4] = pack_bf16(hw[0], hw[1]);
               }
-              if (g16) wst[lane * 4 + (v4 ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+              if (g16) wst[lane * 4 + (((c16 & 1) * 2 + v4) ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
             }
-            if (g16) store_patch(g16, g16_stride, (int64_t)a.I * 4 + (col + half * 32) * 2);
+            if (g16 && (c16 & 1)) store_patch(g16, g16_stride, (int64_t)a.I * 4 + (col + (c16 >> 1) * 32) * 2);
           }
           if (valid && a.dwp) a.dwp[(int64_t)(nt * TC_CG + cg) * a.ld + grow] = dot;
         }
