@@ -54,10 +54,14 @@ constexpr int TC_THREADS = 128 + TC_EPI_THREADS;  // warpgroup 0 = {B producer, 
 #endif
 constexpr int TC_REG_HI = MOE_TC_REG_HI;
 constexpr int TC_REG_LO = TC_CG == 2 ? (64512 - 256 * TC_REG_HI) / 128 : 32;
+constexpr int TC_REG_HI3 = TC_CG == 2 ? 224 : TC_REG_HI;  // MODE 3, whose tile end holds d beside both accumulators
+constexpr int TC_REG_LO3 = TC_CG == 2 ? (64512 - 256 * TC_REG_HI3) / 128 : TC_REG_LO;
 constexpr int TC_REG_LAUNCH = (65536 / TC_THREADS) / 8 * 8;  // what __launch_bounds__(TC_THREADS, 1) lets ptxas use
-static_assert(128 * TC_REG_LO + TC_EPI_THREADS * TC_REG_HI <= TC_THREADS * TC_REG_LAUNCH,
+static_assert(128 * TC_REG_LO + TC_EPI_THREADS * TC_REG_HI <= TC_THREADS * TC_REG_LAUNCH &&
+                  128 * TC_REG_LO3 + TC_EPI_THREADS * TC_REG_HI3 <= TC_THREADS * TC_REG_LAUNCH,
               "setmaxnreg.inc would wait for registers that the CTA's pool never holds");
 constexpr int TC_STAGES = 4;
+constexpr int TC_GRAD_STAGES = 3;           // of the gradients' products (MODE 3 and up)
 constexpr int TC_A_BYTES = 128 * 128;       // 128 rows x 128 B
 constexpr int TC_AR = 16;                   // rows of the small A box ...
 constexpr int TC_AR_BYTES = TC_AR * 128;    // ... which brings just the rows that a short tile has
@@ -78,7 +82,8 @@ struct TcShared {
   int head_item[8];        // expert, first row, end of the expert's rows, n-tile, first K block, K blocks
   float head_w[4];         // weight scales of the item's first two K blocks: (gate|half 0, up|half 1) x 2
   float head_sa[2][128];   // activation scales of the first two K blocks, per row of the tile
-  int head_dst[128];       // bf16 result rows: destination row (or origin tag) of every row of the tile, -1 = no row
+  int head_dst[128];       // bf16 result rows: destination row (or origin tag) of every row of the tile, -1 = no row.  MODE 3,
+                           // which stores none: the rows' routing weights (fp32)
   // results on their way to row-segment stores, one private patch per epilogue warp (down GEMM: 32 rows x 128 B at
   // warp * 4096; gate/up GEMM: 32 rows x 64 B at 4096 + warp * 2048, behind the row maxima that the epilogue's column
   // groups exchange, float [2][TC_CG][128])
@@ -154,6 +159,41 @@ __device__ __forceinline__ float moe_silu_fast(float x) {
   return fmaf(hx, t, hx);
 }
 
+// Pairs of fp32 in one instruction (sm_100): a tile's end is arithmetic, and these take half the issue slots
+__device__ __forceinline__ uint64_t bits2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t bits2(float2 v) { return bits2(v.x, v.y); }
+__device__ __forceinline__ float2 floats2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// sigmoid of two numbers to a few steps of fp32 (the gradient of a routing weight is a sum of fp32 products):
+// 1 / (1 + 2^(-x log2 e)) by the two special-function operations alone.  2^y is 0 below -126 and infinite above 128, the
+// reciprocal of infinity 0.
+__device__ __forceinline__ uint64_t moe_sigmoid2(uint64_t x) {
+  const float2 y = floats2(x);  // (the factor and the 1 below are immediates here; as packed operands they hold registers)
+  float e0, e1, r0, r1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(-1.4426950408889634f * y.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(-1.4426950408889634f * y.y));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(1.f + e0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(1.f + e1));
+  return bits2(r0, r1);
+}
+
 // Instruction descriptor, kind::f8f6f4: D fp32, A/B e4m3, M = 128, N = 256
 __host__ __device__ constexpr uint32_t make_idesc(int b_mn_major) {
   return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((256u >> 3) << 17) | ((128u >> 4) << 24);
@@ -168,6 +208,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs,
                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1, const TcArgs a) {
   constexpr bool GEMM2 = MODE == 1 || MODE == 4, DENSE = MODE == 2 || MODE == 5, GATE_UP = MODE == 0 || MODE == 3;
+  constexpr int STAGES = MODE >= 3 ? TC_GRAD_STAGES : TC_STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcShared* sh = reinterpret_cast<TcShared*>(smem + (size_t)TC_STAGES * TC_STAGE_BYTES);
@@ -176,7 +217,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   volatile int* abort_flag = &sh->abort_flag;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < TC_STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&sh->full[s]), 2);  // the two producers
       mbar_init(smem_u32(&sh->empty[s]), 1);
     }
@@ -203,7 +244,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   // clock 1425 / 1590 MHz; Mixtral shape, 1 token 102.0 / 95.2 us, 32 tokens 277 / 272).
   // Taller tiles take the one 128-row box: four or more small boxes per K block cost more than they saved (DeepSeek
   // shape, 2048 tokens, 64 rows per expert: 2.60 -> 2.70 ms).
-  for (int i = threadIdx.x; i < TC_STAGES * (TC_A_BYTES / 16); i += TC_THREADS)
+  for (int i = threadIdx.x; i < STAGES * (TC_A_BYTES / 16); i += TC_THREADS)
     *reinterpret_cast<uint4*>(smem + (i / (TC_A_BYTES / 16)) * TC_STAGE_BYTES + (i % (TC_A_BYTES / 16)) * 16) = make_uint4(0, 0, 0, 0);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
@@ -258,11 +299,11 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   };
   // results are bf16 rows stored to row_map / row_src destinations (uniform over the launch)
   const bool rows_out = !GATE_UP && MODE != 5 && (a.row_src || (a.KS == 1 && !a.comb32 && !(DENSE && a.out32)));
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_REG_LO));
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MODE == 3 ? TC_REG_LO3 : TC_REG_LO));
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer of the weights (one thread)
     // Two producers, this one for B and warp 3's for A, each on its own clock.  Weights are nobody's output: where the
-    // work list is ready the first TC_STAGES blocks are requested before the kernel in front of this one has finished.
+    // work list is ready the first STAGES blocks are requested before the kernel in front of this one has finished.
     // The waits for a stage to come free begin after it has: their limit covers this kernel's own progress, however long
     // the other one takes.
     if (lane == 0) {
@@ -276,7 +317,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         nx_e = a.mtiles[2 * nx.mt];
       }
       uint32_t s = 0, ph = 1;
-      int ahead = TC_STAGES;  // stages that are free from the start
+      int ahead = STAGES;  // stages that are free from the start
       for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
         const int KB = nx.KB;
         // coordinates of the two boxes of the first K block, and their step per K block
@@ -309,7 +350,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           else tma_load_2d(sb + 128 * 128, DENSE ? &tmB0 : &tmB1, col, row + (DENSE ? 128 : 0), full);
           if (GEMM2) row += kBlock;
           else col += kBlock;
-          if (++s == TC_STAGES) s = 0, ph ^= 1;
+          if (++s == STAGES) s = 0, ph ^= 1;
         }
       }
     }
@@ -333,8 +374,8 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       }
       pdl_wait();  // no operand is complete before that, and the waits' limit is for this kernel alone
       for (uint32_t it = 0; it < n_it; ++it) {
-        const uint32_t s = it % TC_STAGES, buf = it & 1;
-        if (!mbar_wait(smem_u32(&sh->full[s]), (it / TC_STAGES) & 1, abort_flag)) break;
+        const uint32_t s = it % STAGES, buf = it & 1;
+        if (!mbar_wait(smem_u32(&sh->full[s]), (it / STAGES) & 1, abort_flag)) break;
         if (!mbar_wait(smem_u32(&sh->tmem_empty[buf]), ((it >> 1) & 1) ^ 1, abort_flag)) break;
         tc_fence_after();
         // the stage's byte offset, in the descriptors' 16-byte units, stays inside the 14-bit address field
@@ -381,10 +422,13 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (row < row_end) dst[i] = a.row_src ? a.row_src[row] : a.row_map ? a.row_map[row] : row;
         }
       }
-      if (MODE == 3 && lane == 0)  // the item's block of d on its way to L2: its epilogue waits for it with nothing else to do
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<const float4*>(a.dh) + dh_index(w.mt, nI, w.nt, 0, 0, 0, 0)),
-                     "r"((min(row_end - row0, 128) + 31) / 32 * 16384)
-                     : "memory");
+      if (MODE == 3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = row0 + i * 32 + lane;
+          dst[i] = __float_as_int(row >= row_end ? 0.f : a.comb_w ? moe_load_as_f32(a.comb_w, a.row_map[row], a.comb_wdt) : 1.f);
+        }
+      }
       float wv = 0.f;  // lanes 0..3: S0[w0i], S1[w1i], S0[w0i + sstep], S1[w1i + sstep]
       if (lane < 2 || (lane < 4 && w.KB > 1)) wv = scales_of(lane & 1, w.kb0 + (lane >> 1))[((lane & 1) ? w1i : w0i) + ((lane >> 1) ? sstep : 0)];
       // the slot is free once every epilogue warp has taken item n - 1 out of it
@@ -402,7 +446,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       for (int i = 0; i < 4; ++i) sh->head_sa[0][i * 32 + lane] = sa[0][i], sh->head_sa[1][i * 32 + lane] = sa[1][i];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh->head_full));
-      if (rows_out) {
+      if (rows_out || MODE == 3) {
         // (free once every epilogue warp has stored item n - 1: this wait ends at the END of that item, after the
         // head of item n went out above, so neither hand-over holds the other up)
         if (n > 0 && !mbar_wait(smem_u32(&sh->dst_empty), (n - 1) & 1, abort_flag)) {
@@ -446,7 +490,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             tma_load_2d(sa, BOXES ? &tmAs : &tmA, col, row0, full);
             if (BOXES == 2) tma_load_2d(sa + TC_AR_BYTES, &tmAs, col, row0 + TC_AR, full);
             col += kBlock;
-            if (++s == TC_STAGES) s = 0, ph ^= 1;
+            if (++s == STAGES) s = 0, ph ^= 1;
           }
         };
         if (n > 2) k_loop(std::integral_constant<int, 0>{});
@@ -457,7 +501,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   } else if (warp >= 4) {
     pdl_wait();
     // ------------------------------------------------------------------ epilogue (4 * TC_CG warps)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_REG_HI));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MODE == 3 ? TC_REG_HI3 : TC_REG_HI));
     const int q = warp & 3, cg = (warp - 4) >> 2;
     const int rit = q * 32 + lane;  // row inside the tile == TMEM lane
     uint32_t it = 0;
@@ -499,8 +543,22 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const int grow = row0 + rit;
       const bool valid = grow < row_end;
       const bool warp_has_rows = row0 + q * 32 < row_end;  // uniform over the warp
-      float row_w = 1.f;  // MODE 3: the row's routing weight
-      if (MODE == 3 && a.comb_w && valid) row_w = moe_load_as_f32(a.comb_w, a.row_map[grow], a.comb_wdt);
+      // MODE 3: where this thread's d lies in shared memory, 4 columns each (the last four of its 64 do not fit): in the
+      // place of a fourth stage, then behind the patches
+      auto d_stage = [&](int i) {
+        return reinterpret_cast<float4*>(i < 12 ? smem + (size_t)TC_GRAD_STAGES * TC_STAGE_BYTES + (warp - 4) * 6144 + i * 512
+                                                : sh->ostage + 4096 + 8 * 2048 + (warp - 4) * 1536 + (i - 12) * 512) + lane;
+      };
+      if (MODE == 3 && warp_has_rows && ok) {
+        // d is on its way to shared memory while the K loop runs (each thread fetches what it will read; rows that do
+        // not exist become zeros): from global memory at the tile's end, beside the next tile's operands, its latency was
+        // half of that end
+        const float4* src = reinterpret_cast<const float4*>(a.dh) + dh_index(w.mt, a.I / kBlock, nt, q, cg, 0, lane);
+#pragma unroll
+        for (int i = 0; i < 15; ++i)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(d_stage(i))), "l"(src + i * 32), "r"(valid ? 16 : 0)
+                       : "memory");
+      }
       int w0i, w1i;
       scale_index(w, e, w0i, w1i);
       // accumulators as packed fp32 pairs: acc[j][p] = columns (2p, 2p+1) of this thread's TC_CW-column span of half j
@@ -517,7 +575,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         // decode-size batches: most row quarters hold no rows; such a warp only hands every buffer straight back
         clear_acc();
         for (int kb = 0; kb < KB && ok; ++kb, ++it) {
-          if (!mbar_wait(smem_u32(&sh->empty[it % TC_STAGES]), (it / TC_STAGES) & 1, abort_flag)) {
+          if (!mbar_wait(smem_u32(&sh->empty[it % STAGES]), (it / STAGES) & 1, abort_flag)) {
             ok = false;
             break;
           }
@@ -543,7 +601,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             acc[c / TC_CPH][(c % TC_CPH) * (TC_CH / 2) + i] =
                 ffma2(pack2u(sv[2 * i], sv[2 * i + 1]), fp, acc[c / TC_CPH][(c % TC_CPH) * (TC_CH / 2) + i]);
         };
-        if (!mbar_wait(smem_u32(&sh->empty[it % TC_STAGES]), (it / TC_STAGES) & 1, abort_flag)) ok = false;
+        if (!mbar_wait(smem_u32(&sh->empty[it % STAGES]), (it / STAGES) & 1, abort_flag)) ok = false;
         if (ok) {
           tc_fence_after();
           const uint32_t tb = lane_base + (it & 1) * 256;
@@ -570,7 +628,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             tc_ld_issue(chunk_addr(tb, c + 3), s1);
             if (c + 4 < TC_NC) tc_ld_wait(s0, s1);
           }
-          const uint32_t nbar = smem_u32(&sh->empty[(it + 1) % TC_STAGES]), npar = ((it + 1) / TC_STAGES) & 1;
+          const uint32_t nbar = smem_u32(&sh->empty[(it + 1) % STAGES]), npar = ((it + 1) / STAGES) & 1;
           // The last two chunks of this block are in flight.  Is the next block's accumulator there already (it is
           // whenever this warp is what the MMAs wait for)?  Only a test: the buffer goes back before any real wait,
           // or the MMA issuer, which needs this buffer for block kb + 2, would idle until block kb + 1 is done.
@@ -680,50 +738,48 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         };
         uint8_t* const g16 = reinterpret_cast<uint8_t*>(a.g16);
         const int64_t g16_stride = (int64_t)a.I * 6, col = nt * 128 + cg * TC_CW;
-        float amax_u = 0.f, dot = 0.f;
+        float amax_u = 0.f, row_w = 0.f;  // row_w: the row's routing weight
+        uint64_t dot2 = 0;                // sums of h * d over even and odd columns
+        if (mbar_wait(smem_u32(&sh->dst_full), ntile & 1, abort_flag)) {
+          row_w = __int_as_float(sh->head_dst[rit]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh->dst_empty));
+        } else {
+          ok = false;
+        }
         const float4* dsrc = reinterpret_cast<const float4*>(a.dh);
         if (warp_has_rows && ok) {
-          // 16 columns at a time; the next sixteen's d is on the way meanwhile
-          float4 dv[2][4];
-          auto load_d = [&](int c16, float4 (&v)[4]) {
+          const uint64_t w2 = bits2(row_w, row_w);
+          const float4 d_last = valid ? __ldcg(dsrc + dh_index(w.mt, nI3, nt, q, cg, 15, lane)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[i] = valid ? __ldcg(dsrc + dh_index(w.mt, nI3, nt, q, cg, c16 * 4 + i, lane)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          };
-          load_d(0, dv[0]);
-#pragma unroll
-          for (int c16 = 0; c16 < 4; ++c16) {
-            if (c16 < 3) load_d(c16 + 1, dv[(c16 + 1) & 1]);
-#pragma unroll
-            for (int v4 = 0; v4 < 2; ++v4) {
+          for (int c8 = 0; c8 < 8; ++c8) {  // 8 columns at a time
+            {
+              const float4 dv[2] = {*d_stage(c8 * 2), c8 < 7 ? *d_stage(c8 * 2 + 1) : d_last};
               uint32_t ow[4];
 #pragma unroll
               for (int w4 = 0; w4 < 4; ++w4) {
-                const int i = c16 * 8 + v4 * 4 + w4;  // pair of columns
-                const float4 d4 = dv[c16 & 1][v4 * 2 + (w4 >> 1)];
-                const float2 g = unpack2(acc[0][i]), u = unpack2(acc[1][i]);
-                const float d[2] = {(w4 & 1) ? d4.z : d4.x, (w4 & 1) ? d4.w : d4.y}, gg[2] = {g.x, g.y}, uu[2] = {u.x, u.y};
-                float dg[2], du[2], hw[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  const float sg = __fdividef(1.f, 1.f + __expf(-gg[c]));
-                  const float act = gg[c] * sg, h = act * uu[c], dd = row_w * d[c];
-                  dot = fmaf(h, d[c], dot);
-                  dg[c] = dd * uu[c] * fmaf(act, 1.f - sg, sg);
-                  du[c] = dd * act;
-                  hw[c] = row_w * h;
+                const int i = c8 * 4 + w4;  // pair of columns
+                const float4 d4 = dv[w4 >> 1];
+                const uint64_t g = bits2(unpack2(acc[0][i])), u = bits2(unpack2(acc[1][i]));
+                const uint64_t d = (w4 & 1) ? bits2(d4.z, d4.w) : bits2(d4.x, d4.y), wd = mul2(d, w2);
+                const uint64_t sg = moe_sigmoid2(g), act = mul2(g, sg), hh = mul2(act, u);
+                dot2 = fma2(hh, d, dot2);
+                const float2 dg = floats2(mul2(mul2(wd, u), fma2(act, bits2(1.f - floats2(sg).x, 1.f - floats2(sg).y), sg))), du = floats2(mul2(wd, act));
+                acc[0][i] = pack2(dg.x, dg.y);
+                acc[1][i] = pack2(du.x, du.y);
+                amax = fmaxf(amax, fmaxf(fabsf(dg.x), fabsf(dg.y)));
+                amax_u = fmaxf(amax_u, fmaxf(fabsf(du.x), fabsf(du.y)));
+                if (g16) {
+                  const float2 hw = floats2(mul2(hh, w2));
+                  ow[w4] = pack_bf16(hw.x, hw.y);
                 }
-                acc[0][i] = pack2(dg[0], dg[1]);
-                acc[1][i] = pack2(du[0], du[1]);
-                amax = fmaxf(amax, fmaxf(fabsf(dg[0]), fabsf(dg[1])));
-                amax_u = fmaxf(amax_u, fmaxf(fabsf(du[0]), fabsf(du[1])));
-                ow[w4] = pack_bf16(hw[0], hw[1]);
               }
-              if (g16) wst[lane * 4 + (((c16 & 1) * 2 + v4) ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+              if (g16) wst[lane * 4 + ((c8 & 3) ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
             }
-            if (g16 && (c16 & 1)) store_patch(g16, g16_stride, (int64_t)a.I * 4 + (col + (c16 >> 1) * 32) * 2);
+            if (g16 && (c8 & 3) == 3) store_patch(g16, g16_stride, (int64_t)a.I * 4 + (col + (c8 >> 2) * 32) * 2);
           }
-          if (valid && a.dwp) a.dwp[(int64_t)(nt * TC_CG + cg) * a.ld + grow] = dot;
+          if (valid && a.dwp) a.dwp[(int64_t)(nt * TC_CG + cg) * a.ld + grow] = floats2(dot2).x + floats2(dot2).y;
         }
         float* const maxima = reinterpret_cast<float*>(sh->ostage) + (ntile & 1) * (2 * TC_CG * 128);  // [tensor][column half][row]
         maxima[cg * 128 + rit] = amax;
