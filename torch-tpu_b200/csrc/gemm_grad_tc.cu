@@ -34,12 +34,8 @@ namespace {
 
 constexpr int GG_EPI_WARPS = 8;
 constexpr int GG_THREADS = 128 + 32 * GG_EPI_WARPS;
-#ifndef GGS
-#define GGS 5
-#define GGP 2
-#endif
-constexpr int GG_STAGES = GGS;
-constexpr int GG_PATCHES = GGP;
+constexpr int GG_STAGES = 5;
+constexpr int GG_PATCHES = 2;                      // of an epilogue warp: 32 rows x 128 bytes each
 constexpr int GG_BK = 64;
 constexpr int GG_BOX_BYTES = GG_BK * 128;          // an MN-major box: 64 rows of K x 128 bytes
 constexpr int GG_A_BYTES = 128 * GG_BK * 2;        // 16 KB: this CTA's 128 of the tile's 256 rows (M)
@@ -74,6 +70,7 @@ struct GgArgs {
   int K;                   // row product: depth; B's row of step k is k % kb_rows
   int kb_rows;
   int add;                 // results are added to the output (fp32)
+  uint8_t *out0, *out1, *out2;  // the segments' outputs, for groups without rows
   int32_t* status;
 };
 
@@ -110,6 +107,11 @@ __device__ __forceinline__ uint32_t gg_in_cta(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void gg_arrive_expect(uint32_t cluster_bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes) : "memory");
 }
+// after tcgen05 reads (their fence orders them before it): nothing in memory goes with it
+__device__ __forceinline__ void gg_arrive_read(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// with what this CTA's threads wrote to shared memory
 __device__ __forceinline__ void gg_arrive(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -326,23 +328,19 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     uint8_t* const patch0 = patches + (warp - 4) * (GG_PATCHES * GG_PATCH_BYTES);
     const uint32_t tmem_empty_leader = gg_in_cta(smem_u32(&sh->tmem_empty[0]), 0);
     uint32_t n = 0;
-    int stores = 0;
-    bool ok = true;
-    // the patch that the next store takes, once the store before the last has read it
-    auto next_patch = [&]() {
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(GG_PATCHES - 1) : "memory");
+    bool ok = true, zeros = false;  // zeros: the patches hold zeros (and stores may still read them)
+    // both patches, once the stores before have read them
+    auto take_patches = [&]() {
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
-      return reinterpret_cast<uint4*>(patch0 + (stores % GG_PATCHES) * GG_PATCH_BYTES);
+      zeros = false;
+      return reinterpret_cast<uint4*>(patch0);
     };
-    auto send_patch = [&](const CUtensorMap* map, const uint4* patch, int c0, int c1, bool add) {
+    auto patches_written = [&]() {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) {
-        gg_store(map, c0, c1, smem_u32(patch), add);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      }
-      ++stores;
     };
+    auto sent = [&]() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); };
     constexpr int PER = F32 ? 32 : 64;  // columns of a patch
     Item nx{};
     if (pair0 < items) nx = item_of(pair0);
@@ -353,13 +351,28 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const int mrow = w.mt * 256 + rank * 128 + q * 32, row = w.g * a.out_rows + mrow, col0 = w.nt * 256 + cg * 128;
       const bool rows_here = mrow < a.M;
       const int cols = rows_here ? min(128, a.N - col0) : 0;  // columns of this warp that exist
-      if (w.beg >= w.end) {  // an expert without rows
+      if (w.beg >= w.end) {
+        // An expert without rows: zeros, not tile by tile but in runs (the 16 warps of the pair share the item's part of the
+        // expert's matrix, 16-byte units [u, end) each), straight from patches that are cleared once.
         if (!a.add) {
-          for (int c = 0; c < cols; c += PER) {
-            uint4* p = next_patch();
+          if (!zeros) {
+            uint4* p = take_patches();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[lane * 8 + i] = make_uint4(0, 0, 0, 0);
-            send_patch(map, p, col0 + c, row, false);
+            for (int i = 0; i < GG_PATCHES * GG_PATCH_BYTES / 512; ++i) p[i * 32 + lane] = make_uint4(0, 0, 0, 0);
+            patches_written();
+            zeros = true;
+          }
+          if (lane == 0) {
+            const int64_t units = (int64_t)a.M * a.N * (F32 ? 4 : 2) / 16, parts = (int64_t)a.MT * a.NT * 2 * GG_EPI_WARPS;
+            const int64_t i = ((int64_t)w.mt * a.NT + w.nt) * 2 * GG_EPI_WARPS + rank * GG_EPI_WARPS + (warp - 4);
+            int64_t u = units * i / parts;
+            const int64_t end = units * (i + 1) / parts;
+            uint8_t* base = (w.seg == 0 ? a.out0 : w.seg == 1 ? a.out1 : a.out2) + (int64_t)w.g * units * 16;
+            for (; u < end; u += GG_PATCHES * GG_PATCH_BYTES / 16)
+              asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + u * 16), "r"(smem_u32(patch0)),
+                           "r"((uint32_t)(min(end - u, (int64_t)(GG_PATCHES * GG_PATCH_BYTES / 16)) * 16))
+                           : "memory");
+            sent();
           }
         }
         continue;
@@ -369,7 +382,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       auto release = [&](uint32_t buf) {  // the accumulator is in registers (or nobody wants it)
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) gg_arrive(tmem_empty_leader + buf * 8);
+        if (lane == 0) gg_arrive_read(tmem_empty_leader + buf * 8);
       };
       if constexpr (F32) {
         float acc[128];
@@ -399,14 +412,23 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < 128; c += PER) {
-          if (c >= cols) break;
-          uint4* p = next_patch();
+        for (int c0 = 0; c0 < 128; c0 += GG_PATCHES * PER) {  // both patches at a time: one fence, two stores
+          if (c0 >= cols) break;
+          uint4* p = take_patches();
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            put(p, i, make_uint4(__float_as_uint(acc[c + 4 * i]), __float_as_uint(acc[c + 4 * i + 1]), __float_as_uint(acc[c + 4 * i + 2]),
-                                 __float_as_uint(acc[c + 4 * i + 3])));
-          send_patch(map, p, col0 + c, row, a.add);
+          for (int h = 0; h < GG_PATCHES; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int c = c0 + h * PER + 4 * i;
+              put(p + h * (GG_PATCH_BYTES / 16), i, make_uint4(__float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]),
+                                                               __float_as_uint(acc[c + 3])));
+            }
+          patches_written();
+          if (lane == 0) {
+            gg_store(map, col0 + c0, row, smem_u32(p), a.add);
+            if (c0 + PER < cols) gg_store(map, col0 + c0 + PER, row, smem_u32(p) + GG_PATCH_BYTES, a.add);
+            sent();
+          }
         }
       } else {
         const uint32_t buf = n & 1;
@@ -424,26 +446,38 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         // all 128 columns leave tensor memory before the first store, so that the accumulator goes back early
         uint32_t o[64];
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t v0[16], v1[16];
+        for (int c = 0; c < 128; c += 64) {
+          uint32_t v0[16], v1[16], v2[16], v3[16];
           tc_ld_issue(tb + c, v0);
           tc_ld_issue(tb + c + 16, v1);
+          tc_ld_issue(tb + c + 32, v2);
+          tc_ld_issue(tb + c + 48, v3);
           tc_ld_wait(v0, v1);
+          tc_ld_wait(v2, v3);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             o[c / 2 + i] = pack(v0[2 * i], v0[2 * i + 1]);
             o[c / 2 + 8 + i] = pack(v1[2 * i], v1[2 * i + 1]);
+            o[c / 2 + 16 + i] = pack(v2[2 * i], v2[2 * i + 1]);
+            o[c / 2 + 24 + i] = pack(v3[2 * i], v3[2 * i + 1]);
           }
         }
         release(buf);
+        if (cols > 0) {
+          uint4* p = take_patches();
 #pragma unroll
-        for (int c = 0; c < 128; c += PER) {
-          if (c >= cols) break;
-          uint4* p = next_patch();
+          for (int h = 0; h < GG_PATCHES; ++h)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            put(p, i, make_uint4(o[c / 2 + 4 * i], o[c / 2 + 4 * i + 1], o[c / 2 + 4 * i + 2], o[c / 2 + 4 * i + 3]));
-          send_patch(map, p, col0 + c, row, false);
+            for (int i = 0; i < 8; ++i) {
+              const int c = (h * PER) / 2 + 4 * i;
+              put(p + h * (GG_PATCH_BYTES / 16), i, make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]));
+            }
+          patches_written();
+          if (lane == 0) {
+            gg_store(map, col0, row, smem_u32(p), false);
+            if (PER < cols) gg_store(map, col0 + PER, row, smem_u32(p) + GG_PATCH_BYTES, false);
+            sent();
+          }
         }
       }
     }
@@ -512,6 +546,7 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   a.M = g.M, a.N = g.N;
   a.MT = (g.M + 255) / 256, a.NT = (g.N + 255) / 256;
   a.out_rows = g.M;
+  a.out0 = reinterpret_cast<uint8_t*>(g.out[0]), a.out1 = reinterpret_cast<uint8_t*>(g.out[1]), a.out2 = reinterpret_cast<uint8_t*>(g.out[2]);
   a.add = g.add;
   a.status = g.status;
   return g.out_f32 ? gg_launch<false, true>(tm, a, st) : gg_launch<false, false>(tm, a, st);
