@@ -117,6 +117,7 @@ constexpr int CG_THREADS = 256;
 constexpr int CG_VEC = 4;                            // 16-byte pieces of a row per thread
 constexpr int CG_COLS = CG_THREADS * 8 * CG_VEC;     // 8192
 constexpr int CG_MAXK = 32;
+constexpr int CG_SLOTS = 2;
 __global__ void __launch_bounds__(CG_THREADS)
 combine_grad_kernel(__nv_bfloat16* dy, float* dw, const __nv_bfloat16* dout, const __nv_bfloat16* y, const void* w, int w_dtype,
                     const int32_t* ids, int E, int k, int H) {
@@ -132,31 +133,42 @@ combine_grad_kernel(__nv_bfloat16* dy, float* dw, const __nv_bfloat16* dout, con
       col[u] = c0 + (u * CG_THREADS + threadIdx.x) * 8;
       d[u] = col[u] < H ? *reinterpret_cast<const uint4*>(dout + t * H + col[u]) : make_uint4(0, 0, 0, 0);
     }
-    for (int j = 0; j < k; ++j) {
-      const int64_t p = t * k + j;
-      const bool on = !(ids && (ids[p] < 0 || ids[p] >= E));  // (a dropped slot: its row of y was never written)
-      const float wj = dy && on ? moe_load_as_f32(w, p, w_dtype) : 0.f;
-      uint4 yv[CG_VEC];
+    // Two slots at a time, their loads issued before the first store (which could be to the row that the next load reads,
+    // for all the compiler knows)
+    for (int j0 = 0; j0 < k; j0 += CG_SLOTS) {
+      bool on[CG_SLOTS];
+      float wj[CG_SLOTS];
+      uint4 yv[CG_SLOTS][CG_VEC];
 #pragma unroll
-      for (int u = 0; u < CG_VEC; ++u)
-        yv[u] = dw && on && col[u] < H ? *reinterpret_cast<const uint4*>(y + p * H + col[u]) : make_uint4(0, 0, 0, 0);
-      float dot = 0.f;
+      for (int s = 0; s < CG_SLOTS; ++s) {
+        const int64_t p = t * k + j0 + s;
+        on[s] = j0 + s < k && !(ids && (ids[p] < 0 || ids[p] >= E));  // (a dropped slot: its row of y was never written)
+        wj[s] = dy && on[s] ? moe_load_as_f32(w, p, w_dtype) : 0.f;
 #pragma unroll
-      for (int u = 0; u < CG_VEC; ++u) {
-        if (col[u] >= H) continue;
-        const __nv_bfloat162 *d2 = reinterpret_cast<const __nv_bfloat162*>(&d[u]), *y2 = reinterpret_cast<const __nv_bfloat162*>(&yv[u]);
-        uint4 o;
-        __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 df = __bfloat1622float2(d2[i]), yf = __bfloat1622float2(y2[i]);
-          if (on) dot = fmaf(df.x, yf.x, fmaf(df.y, yf.y, dot));
-          o2[i] = on ? __floats2bfloat162_rn(wj * df.x, wj * df.y) : __floats2bfloat162_rn(0.f, 0.f);
-        }
-        if (dy) *reinterpret_cast<uint4*>(dy + p * H + col[u]) = o;
+        for (int u = 0; u < CG_VEC; ++u)
+          yv[s][u] = dw && on[s] && col[u] < H ? *reinterpret_cast<const uint4*>(y + p * H + col[u]) : make_uint4(0, 0, 0, 0);
       }
-      dot = warp_sum(dot);
-      if (lane == 0) part[warp][j] = (c0 ? part[warp][j] : 0.f) + dot;
+#pragma unroll
+      for (int s = 0; s < CG_SLOTS; ++s) {
+        if (j0 + s >= k) break;
+        float dot = 0.f;
+#pragma unroll
+        for (int u = 0; u < CG_VEC; ++u) {
+          if (col[u] >= H) continue;
+          const __nv_bfloat162 *d2 = reinterpret_cast<const __nv_bfloat162*>(&d[u]), *y2 = reinterpret_cast<const __nv_bfloat162*>(&yv[s][u]);
+          uint4 o;
+          __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 df = __bfloat1622float2(d2[i]), yf = __bfloat1622float2(y2[i]);
+            if (on[s]) dot = fmaf(df.x, yf.x, fmaf(df.y, yf.y, dot));
+            o2[i] = on[s] ? __floats2bfloat162_rn(wj[s] * df.x, wj[s] * df.y) : __floats2bfloat162_rn(0.f, 0.f);
+          }
+          if (dy) *reinterpret_cast<uint4*>(dy + (t * k + j0 + s) * H + col[u]) = o;
+        }
+        dot = warp_sum(dot);
+        if (lane == 0) part[warp][j0 + s] = (c0 ? part[warp][j0 + s] : 0.f) + dot;
+      }
     }
   }
   __syncthreads();
@@ -260,14 +272,24 @@ __global__ void __launch_bounds__(256)
 grad_finish_kernel(const FinishArgs a) {
   pdl_begin();
   if (blockIdx.x >= a.dx_blocks) {
-    const int64_t r = ((int64_t)blockIdx.x - a.dx_blocks) * 256 + threadIdx.x, P = a.T * a.k;
-    if (r >= P) return;
-    if (a.pos_of[r] < 0) a.dw[r] = 0.f;
-    const int pair = a.sorted[r];
-    if (pair < 0) return;
+    // 32 rows to a block; its eight warps sum an eighth of the parts each, in order, and the first adds the eight up
+    __shared__ float eighth[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t r = ((int64_t)blockIdx.x - a.dx_blocks) * 32 + lane, P = a.T * a.k;
+    const int pair = r < P ? a.sorted[r] : -1;
     float s = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < a.parts; ++i) s += a.dwp[(int64_t)i * a.ld + r];
+    if (pair >= 0) {
+      const int end = a.parts * (warp + 1) / 8;
+#pragma unroll 4
+      for (int i = a.parts * warp / 8; i < end; ++i) s += a.dwp[(int64_t)i * a.ld + r];
+    }
+    eighth[warp][lane] = s;
+    __syncthreads();
+    if (warp > 0 || r >= P) return;
+    if (a.pos_of[r] < 0) a.dw[r] = 0.f;  // pair r was dropped
+    if (pair < 0) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += eighth[i][lane];
     a.dw[pair] = s;
     return;
   }
@@ -371,6 +393,43 @@ router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int
   }
 }
 
+// A few tokens: both products in one kernel on the CUDA cores.  A block owns 32 columns of H: the tokens' and the
+// router's columns and dlogits as fp32 in shared memory; a thread owns a column and every eighth token and expert.  fp32
+// sums in order.
+constexpr int RGS_COLS = 32, RGS_THREADS = 256, RGS_ROWS = RGS_THREADS / RGS_COLS;
+constexpr int RGS_MAX_T = 64, RGS_MAX_TE = 8192;  // tokens, tokens x experts
+__global__ void __launch_bounds__(RGS_THREADS)
+router_small_grad_kernel(__nv_bfloat16* dx, void* dwr, int f32, int add, const float* dlogits, const __nv_bfloat16* x,
+                         const __nv_bfloat16* wr, int T, int H, int E) {
+  pdl_begin();
+  extern __shared__ float rgs[];
+  float *dl = rgs, *xs = dl + T * E, *ws = xs + (x ? T * RGS_COLS : 0);  // [T][E], [T][COLS], [E][COLS]
+  const int h0 = blockIdx.x * RGS_COLS, c = threadIdx.x % RGS_COLS, r = threadIdx.x / RGS_COLS, h = h0 + c;
+  for (int i = threadIdx.x; i < T * E; i += RGS_THREADS) dl[i] = dlogits[i];
+  if (x)
+    for (int t = r; t < T; t += RGS_ROWS) xs[t * RGS_COLS + c] = h < H ? __bfloat162float(x[(int64_t)t * H + h]) : 0.f;
+  if (dx)
+    for (int e = r; e < E; e += RGS_ROWS) ws[e * RGS_COLS + c] = h < H ? __bfloat162float(wr[(int64_t)e * H + h]) : 0.f;
+  __syncthreads();
+  if (h >= H) return;
+  if (dx)
+    for (int t = r; t < T; t += RGS_ROWS) {
+      float s = 0.f;
+#pragma unroll 8
+      for (int e = 0; e < E; ++e) s = fmaf(dl[t * E + e], ws[e * RGS_COLS + c], s);
+      dx[(int64_t)t * H + h] = __float2bfloat16_rn(s);
+    }
+  if (x)
+    for (int e = r; e < E; e += RGS_ROWS) {
+      float s = 0.f;
+#pragma unroll 8
+      for (int t = 0; t < T; ++t) s = fmaf(dl[t * E + e], xs[t * RGS_COLS + c], s);
+      const int64_t at = (int64_t)e * H + h;
+      if (f32) reinterpret_cast<float*>(dwr)[at] = add ? reinterpret_cast<float*>(dwr)[at] + s : s;
+      else reinterpret_cast<__nv_bfloat16*>(dwr)[at] = __float2bfloat16_rn(s);
+    }
+}
+
 __global__ void grad_scales_kernel(float* __restrict__ dst, const __nv_bfloat16* a, const __nv_bfloat16* b, const __nv_bfloat16* c,
                                    int64_t n) {  // block scales in fp32: dst = a | b | c (b, c may be NULL)
   pdl_begin();
@@ -467,6 +526,21 @@ extern "C" int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype
   if ((dx && !(moe_aligned16(dx) && moe_aligned16(wr))) || (dwr && !(moe_aligned16(dwr) && moe_aligned16(x)))) return B200MOE_EALIGN;
   if (!moe_tc_available()) return B200MOE_EDRIVER;
   const RouterLayout L = router_layout(T, H, E);
+  if (T <= RGS_MAX_T && T * E <= RGS_MAX_TE) {
+    const size_t smem = sizeof(float) * (size_t)(T * E + (dwr ? T * RGS_COLS : 0) + (dx ? E * RGS_COLS : 0));
+    static bool attr_set[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200MOE_EDRIVER;
+    if (!attr_set[dev]) {  // per-device attribute; the most there can be: T * E, T and E at their limits
+      cudaFuncSetAttribute(router_small_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)sizeof(float) * (RGS_MAX_TE + (RGS_MAX_T + 1024) * RGS_COLS));
+      attr_set[dev] = true;
+    }
+    return moe_launch(router_small_grad_kernel, (unsigned)((H + RGS_COLS - 1) / RGS_COLS), RGS_THREADS, smem, st,
+                      reinterpret_cast<__nv_bfloat16*>(dx), dwr, (int)(dwr_dtype == B200MOE_F32), accumulate, dlogits,
+                      reinterpret_cast<const __nv_bfloat16*>(dwr ? x : nullptr), reinterpret_cast<const __nv_bfloat16*>(wr), (int)T, (int)H,
+                      (int)E);
+  }
   if (!workspace || workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return B200MOE_EWORKSPACE;
   char* ws = reinterpret_cast<char*>(workspace);
   __nv_bfloat16* split = reinterpret_cast<__nv_bfloat16*>(ws + L.split);
@@ -803,7 +877,7 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
     f.T = d->T, f.ld = L.ld;
     f.dx_blocks = dx ? (d->T * (d->H / 8) + 255) / 256 : 0;
     f.E = (int)d->E, f.k = (int)d->k, f.H = (int)d->H, f.parts = (int)(d->I / 64);
-    rc = moe_launch(grad_finish_kernel, (unsigned)(f.dx_blocks + (dw ? (L.P + 255) / 256 : 0)), 256, 0, st, f);
+    rc = moe_launch(grad_finish_kernel, (unsigned)(f.dx_blocks + (dw ? (L.P + 31) / 32 : 0)), 256, 0, st, f);
   }
   return rc;
 }

@@ -1,6 +1,7 @@
 """Functional wrappers over the C ABI taking torch CUDA tensors (device memory and streams are torch's;
 the arithmetic is all in libb200moe).  Every function enqueues on torch's current stream and returns
 without synchronising.  Inputs must be contiguous CUDA tensors; nothing here falls back to PyTorch math."""
+import contextlib
 import ctypes
 
 import torch
@@ -258,20 +259,21 @@ def linear_w8(x, w, scale, out=None, workspace=None, status=None):
 # layer.FusedMoE.backward does.  All tensors of a call are on one device, which need not be the current one.
 
 def _chk_grad(t, name, dtypes, shape, device):
+    if (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == shape and t.device == device and device.type == "cuda"
+            and t.is_contiguous()):
+        return
     _chk(t, name)
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
-    dtypes = dtypes if isinstance(dtypes, tuple) else (dtypes,)
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _grad_out(t, name, dtypes, shape, device):
     """`t`, checked, or a new tensor of the first of `dtypes`."""
     if t is None:
-        return torch.empty(shape, dtype=dtypes[0] if isinstance(dtypes, tuple) else dtypes, device=device)
+        return torch.empty(shape, dtype=dtypes[0], device=device)
     _chk_grad(t, name, dtypes, shape, device)
     return t
 
@@ -281,20 +283,38 @@ def _rank(t, name, dims):
         raise ValueError(f"{name} must be a tensor of {dims} dimensions")
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on(device):
+    """The calls below launch on the current device: the tensors' one, for their time."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _raw_stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
 def _workspace(workspace, need, what, device):
     if need == 0:
         raise ValueError(f"unsupported sizes for {what} (see include/b200moe.h)")
     if workspace is None:
         workspace = torch.empty(need + 256, dtype=torch.uint8, device=device)
-    elif workspace.device != device:
-        raise ValueError(f"workspace must be on {device}, got {workspace.device}")
+    else:
+        _chk(workspace, "workspace")
+        if workspace.device != device:
+            raise ValueError(f"workspace must be on {device}, got {workspace.device}")
     base = (workspace.data_ptr() + 255) // 256 * 256
-    return workspace, ctypes.c_void_p(base), workspace.numel() * workspace.element_size() - (base - workspace.data_ptr())
+    return workspace, base, workspace.numel() * workspace.element_size() - (base - workspace.data_ptr())
 
 
 def _chk_status(status, device):
     if status is not None:
-        _chk_grad(status, "status", torch.int32, status.shape, device)
+        _chk_grad(status, "status", _I32, status.shape, device)
 
 
 def _chk_accumulate(accumulate, t, name):
@@ -302,6 +322,7 @@ def _chk_accumulate(accumulate, t, name):
         raise ValueError(f"accumulate needs fp32 {name} to add to")
 
 
+_F32, _BF16, _I32, _E4M3 = (torch.float32,), (torch.bfloat16,), (torch.int32,), (torch.float8_e4m3fn,)
 _GRAD = (torch.float32, torch.bfloat16)
 
 
@@ -312,18 +333,18 @@ def route_backward(dw, logits, ids, score_func="softmax", renorm=True, scale=1.0
     _rank(logits, "logits", 2)
     _rank(ids, "ids", 2)
     dev, (T, E), k = logits.device, logits.shape, ids.shape[1]
-    _chk_grad(logits, "logits", torch.float32, (T, E), dev)
-    _chk_grad(ids, "ids", torch.int32, (T, k), dev)
+    _chk_grad(logits, "logits", _F32, (T, E), dev)
+    _chk_grad(ids, "ids", _I32, (T, k), dev)
     _chk_grad(dw, "dw", _GRAD, (T, k), dev)
     if logit_bias is not None:
-        _chk_grad(logit_bias, "logit_bias", torch.float32, (E,), dev)
+        _chk_grad(logit_bias, "logit_bias", _F32, (E,), dev)
     if score_func not in ("softmax", "sigmoid"):
         raise ValueError(f"score_func must be softmax or sigmoid, got {score_func!r}")
-    with torch.cuda.device(dev):
-        dlogits = _grad_out(dlogits, "dlogits", torch.float32, (T, E), dev)
+    with _on(dev):
+        dlogits = _grad_out(dlogits, "dlogits", _F32, (T, E), dev)
         sf = L.SCORE_SOFTMAX if score_func == "softmax" else L.SCORE_SIGMOID
-        L.check(L.lib().b200moe_route_backward(_ptr(dlogits), _ptr(logits), _ptr(logit_bias), _ptr(ids), _ptr(dw), _DT[dw.dtype],
-                                               T, E, k, sf, int(renorm), float(scale), _stream()), "b200moe_route_backward")
+        L.check(L.lib().b200moe_route_backward(_addr(dlogits), _addr(logits), _addr(logit_bias), _addr(ids), _addr(dw), _DT[dw.dtype],
+                                               T, E, k, sf, int(renorm), float(scale), _raw_stream(dev)), "b200moe_route_backward")
     return dlogits
 
 
@@ -335,21 +356,21 @@ def router_logits_backward(dlogits, x=None, wr=None, dx=None, dwr=None, accumula
         raise ValueError("x or wr is needed")
     _rank(x if x is not None else wr, "x" if x is not None else "wr", 2)
     dev, (T, E), H = dlogits.device, dlogits.shape, (x if x is not None else wr).shape[1]
-    _chk_grad(dlogits, "dlogits", torch.float32, (T, E), dev)
+    _chk_grad(dlogits, "dlogits", _F32, (T, E), dev)
     if x is not None:
-        _chk_grad(x, "x", torch.bfloat16, (T, H), dev)
+        _chk_grad(x, "x", _BF16, (T, H), dev)
         _chk_accumulate(accumulate, dwr, "dwr")
     if wr is not None:
-        _chk_grad(wr, "wr", torch.bfloat16, (E, H), dev)
+        _chk_grad(wr, "wr", _BF16, (E, H), dev)
     _chk_status(status, dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         need = L.lib().b200moe_router_logits_backward_workspace_bytes(T, H, E)
         keep, base, avail = _workspace(workspace, need, "b200moe_router_logits_backward", dev)
-        dx = _grad_out(dx, "dx", torch.bfloat16, (T, H), dev) if wr is not None else None
+        dx = _grad_out(dx, "dx", _BF16, (T, H), dev) if wr is not None else None
         dwr = _grad_out(dwr, "dwr", _GRAD, (E, H), dev) if x is not None else None
-        L.check(L.lib().b200moe_router_logits_backward(_ptr(dx), _ptr(dwr), _DT[dwr.dtype] if dwr is not None else L.F32,
-                                                       int(accumulate and dwr is not None), _ptr(dlogits), _ptr(x), _ptr(wr), T, H, E,
-                                                       base, avail, _ptr(status), _stream()), "b200moe_router_logits_backward")
+        L.check(L.lib().b200moe_router_logits_backward(_addr(dx), _addr(dwr), _DT[dwr.dtype] if dwr is not None else L.F32,
+                                                       int(accumulate and dwr is not None), _addr(dlogits), _addr(x), _addr(wr), T, H, E,
+                                                       base, avail, _addr(status), _raw_stream(dev)), "b200moe_router_logits_backward")
     return dx, dwr
 
 
@@ -359,16 +380,16 @@ def combine_backward(dout, y, w, ids=None, num_experts=0, dy=None, dw=None):
     masks them the same way).  ``dy`` may be ``y`` itself.  The gradient of ``add`` is dout."""
     _rank(y, "y", 3)
     dev, (T, k, H) = y.device, y.shape
-    _chk_grad(y, "y", torch.bfloat16, (T, k, H), dev)
-    _chk_grad(dout, "dout", torch.bfloat16, (T, H), dev)
+    _chk_grad(y, "y", _BF16, (T, k, H), dev)
+    _chk_grad(dout, "dout", _BF16, (T, H), dev)
     _chk_grad(w, "w", (torch.float32, torch.bfloat16, torch.float16), (T, k), dev)
     if ids is not None:
-        _chk_grad(ids, "ids", torch.int32, (T, k), dev)
-    with torch.cuda.device(dev):
-        dy = _grad_out(dy, "dy", torch.bfloat16, (T, k, H), dev)
-        dw = _grad_out(dw, "dw", torch.float32, (T, k), dev)
-        L.check(L.lib().b200moe_combine_backward(_ptr(dy), _ptr(dw), _ptr(dout), _ptr(y), _ptr(w), _DT[w.dtype], _ptr(ids), num_experts,
-                                                 T, k, H, _stream()), "b200moe_combine_backward")
+        _chk_grad(ids, "ids", _I32, (T, k), dev)
+    with _on(dev):
+        dy = _grad_out(dy, "dy", _BF16, (T, k, H), dev)
+        dw = _grad_out(dw, "dw", _F32, (T, k), dev)
+        L.check(L.lib().b200moe_combine_backward(_addr(dy), _addr(dw), _addr(dout), _addr(y), _addr(w), _DT[w.dtype], _addr(ids), num_experts,
+                                                 T, k, H, _raw_stream(dev)), "b200moe_combine_backward")
     return dy, dw
 
 
@@ -381,24 +402,24 @@ def linear_w8_backward(dy, x=None, w=None, scale=None, dx=None, dw=None, accumul
         raise ValueError("x or w is needed")
     _rank(x if x is not None else w, "x" if x is not None else "w", 2)
     dev, (M, N), K = dy.device, dy.shape, (x if x is not None else w).shape[1]
-    _chk_grad(dy, "dy", torch.bfloat16, (M, N), dev)
+    _chk_grad(dy, "dy", _BF16, (M, N), dev)
     if x is not None:
-        _chk_grad(x, "x", torch.bfloat16, (M, K), dev)
+        _chk_grad(x, "x", _BF16, (M, K), dev)
         _chk_accumulate(accumulate, dw, "dw")
     if w is not None:
-        _chk_grad(w, "w", torch.float8_e4m3fn, (N, K), dev)
+        _chk_grad(w, "w", _E4M3, (N, K), dev)
         _chk_grad(scale, "scale", _GRAD, ((N + 127) // 128, (K + 127) // 128), dev)
     _chk_status(status, dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         sdt = _DT[scale.dtype] if w is not None else L.F32
         need = L.lib().b200moe_linear_w8_backward_workspace_bytes(M, K, N, sdt)
         keep, base, avail = _workspace(workspace, need, "b200moe_linear_w8_backward", dev)
-        dx = _grad_out(dx, "dx", torch.bfloat16, (M, K), dev) if w is not None else None
+        dx = _grad_out(dx, "dx", _BF16, (M, K), dev) if w is not None else None
         dw = _grad_out(dw, "dw", _GRAD, (N, K), dev) if x is not None else None
-        L.check(L.lib().b200moe_linear_w8_backward(_ptr(dx), _ptr(dw), _DT[dw.dtype] if dw is not None else L.F32,
-                                                   int(accumulate and dw is not None), _ptr(dy), _ptr(x), _ptr(w),
-                                                   _ptr(scale) if w is not None else _ptr(None), sdt, M, K, N, base, avail,
-                                                   _ptr(status), _stream()), "b200moe_linear_w8_backward")
+        L.check(L.lib().b200moe_linear_w8_backward(_addr(dx), _addr(dw), _DT[dw.dtype] if dw is not None else L.F32,
+                                                   int(accumulate and dw is not None), _addr(dy), _addr(x), _addr(w),
+                                                   _addr(scale) if w is not None else None, sdt, M, K, N, base, avail,
+                                                   _addr(status), _raw_stream(dev)), "b200moe_linear_w8_backward")
     return dx, dw
 
 
@@ -425,15 +446,15 @@ def experts_backward(dout, x, wg, wu, wd, sg, su, sd, ids, topk_w=None, *, dx=No
     _rank(wg, "wg", 3)
     _rank(ids, "ids", 2)
     dev, (T, H), (E, I, _), k = x.device, x.shape, wg.shape, ids.shape[1]
-    _chk_grad(x, "x", torch.bfloat16, (T, H), dev)
-    _chk_grad(ids, "ids", torch.int32, (T, k), dev)
+    _chk_grad(x, "x", _BF16, (T, H), dev)
+    _chk_grad(ids, "ids", _I32, (T, k), dev)
     for n, t in (("wg", wg), ("wu", wu), ("wd", wd)):
-        _chk_grad(t, n, torch.float8_e4m3fn, (E, I, H), dev)
+        _chk_grad(t, n, _E4M3, (E, I, H), dev)
     for n, t in (("sg", sg), ("su", su), ("sd", sd)):
-        _chk_grad(t, n, sg.dtype if isinstance(sg, torch.Tensor) and sg.dtype in _GRAD else _GRAD,
+        _chk_grad(t, n, (sg.dtype,) if isinstance(sg, torch.Tensor) and sg.dtype in _GRAD else _GRAD,
                   (E, (I + 127) // 128, (H + 127) // 128), dev)
     per_slot = isinstance(dout, torch.Tensor) and dout.dim() == 3
-    _chk_grad(dout, "dout", torch.bfloat16, (T, k, H) if per_slot else (T, H), dev)
+    _chk_grad(dout, "dout", _BF16, (T, k, H) if per_slot else (T, H), dev)
     if per_slot:
         if topk_w is not None or dw is not None:
             raise ValueError("per-slot dout goes with un-weighted rows: topk_w and dw must be None")
@@ -442,27 +463,27 @@ def experts_backward(dout, x, wg, wu, wd, sg, su, sd, ids, topk_w=None, *, dx=No
             raise ValueError("topk_w is needed (dout [T,H] is the gradient of the weighted combine)")
         _chk_grad(topk_w, "topk_w", _GRAD, (T, k), dev)
     if add is not None:
-        _chk_grad(add, "add", torch.bfloat16, (T, H), dev)
+        _chk_grad(add, "add", _BF16, (T, H), dev)
     if weight_grads is not None:
         if len(weight_grads) != 3:
             raise ValueError("weight_grads is (dwg, dwu, dwd)")
         for n, t in zip(("dwg", "dwu", "dwd"), weight_grads):
-            _chk_grad(t, n, weight_grads[0].dtype if weight_grads[0].dtype in _GRAD else _GRAD, (E, I, H), dev)
+            _chk_grad(t, n, (weight_grads[0].dtype,) if weight_grads[0].dtype in _GRAD else _GRAD, (E, I, H), dev)
             _chk_accumulate(accumulate, t, n)
     _chk_status(status, dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         d = make_backward_desc(T, H, I, E, k, per_slot=per_slot, scale_dtype=sg.dtype,
                                w_dtype=topk_w.dtype if topk_w is not None else torch.float32, weight_grads=weight_grads is not None,
                                grad_dtype=weight_grads[0].dtype if weight_grads is not None else torch.float32,
                                accumulate=accumulate and weight_grads is not None)
         keep, base, avail = _workspace(workspace, experts_backward_workspace_bytes(d), "b200moe_experts_backward", dev)
-        dx = _grad_out(dx, "dx", torch.bfloat16, (T, H), dev)
+        dx = _grad_out(dx, "dx", _BF16, (T, H), dev)
         if not per_slot:
-            dw = _grad_out(dw, "dw", torch.float32, (T, k), dev)
-        g = [_ptr(t) for t in weight_grads] if weight_grads is not None else [ctypes.c_void_p(0)] * 3
-        L.check(L.lib().b200moe_experts_backward(_ptr(dx), _ptr(dw), *g, _ptr(dout), _ptr(x), _ptr(wg), _ptr(wu), _ptr(wd), _ptr(sg),
-                                                 _ptr(su), _ptr(sd), _ptr(ids), _ptr(topk_w), _ptr(add), ctypes.byref(d), base, avail,
-                                                 _ptr(status), _stream()), "b200moe_experts_backward")
+            dw = _grad_out(dw, "dw", _F32, (T, k), dev)
+        g = [_addr(t) for t in weight_grads] if weight_grads is not None else [None] * 3
+        L.check(L.lib().b200moe_experts_backward(_addr(dx), _addr(dw), *g, _addr(dout), _addr(x), _addr(wg), _addr(wu), _addr(wd), _addr(sg),
+                                                 _addr(su), _addr(sd), _addr(ids), _addr(topk_w), _addr(add), ctypes.byref(d), base, avail,
+                                                 _addr(status), _raw_stream(dev)), "b200moe_experts_backward")
     return dx, dw
 
 
