@@ -67,6 +67,7 @@ struct GgArgs {
   int P, groups, segs;     // segs: operand pairs that a group has (columns [seg * M, (seg + 1) * M) of A)
   int M, N, MT, NT;        // outputs of one (group, segment); tiles along both
   int out_rows;            // rows of the output between groups
+  int kparts, kpart_cols;  // the K range is walked kparts times, with columns of A kpart_cols further each time
   int K;                   // row product: depth; B's row of step k is k % kb_rows
   int kb_rows;
   int add;                 // results are added to the output (fp32)
@@ -208,9 +209,11 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   // rows of the item's last K step, if some of the rows that its MMAs read there are not the group's (0: none are)
   auto tail_rows = [&](const Item& w) {
     const int last = (w.end - w.beg) & (GG_BK - 1);
-    return !ROWS && w.end < a.P && (last & 15) ? last : 0;
+    return !ROWS && a.kparts == 1 && w.end < a.P && (last & 15) ? last : 0;
   };
-  auto piece = [&](const Item& w) { return F32 && !ROWS ? kGradChunk : max(w.end - w.beg, 1); };
+  auto steps_once = [&](const Item& w) { return (max(w.end - w.beg, 0) + GG_BK - 1) / GG_BK; };
+  // K steps that one accumulator takes
+  auto piece = [&](int steps) { return F32 && !ROWS ? kGradChunk / GG_BK : steps; };
 
   if (F32 && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GG_REG_LO));
   if (warp == 0) {
@@ -226,8 +229,9 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const CUtensorMap* tmB = w.seg == 2 ? &tmB1 : &tmB0;
         const int m0 = w.mt * 256 + rank * 128, n0 = w.nt * 256 + rank * 128;
         const bool tail = tail_rows(w) != 0;
-        int brow = w.beg;
-        for (int r = w.beg; r < w.end; r += GG_BK) {
+        const int once = steps_once(w), steps = once * a.kparts;
+        int r = w.beg, brow = w.beg, acol = ROWS ? 0 : w.seg * a.M + m0, left = once;
+        for (int i = 0; i < steps; ++i) {
           if (!mbar_wait(smem_u32(&sh->empty[0]) + s * 8, ph, abort_flag)) {
             ok = false;
             break;
@@ -240,13 +244,14 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (ROWS) {
             gg_load(sa, &tmA, r, m0, bar);
           } else {
-            gg_load(sa, &tmA, w.seg * a.M + m0, r, bar);
-            gg_load(sa + GG_BOX_BYTES, &tmA, w.seg * a.M + m0 + 64, r, bar);
+            gg_load(sa, &tmA, acol, r, bar);
+            gg_load(sa + GG_BOX_BYTES, &tmA, acol + 64, r, bar);
           }
           gg_load(sb, tmB, n0, brow, bar);
           gg_load(sb + GG_BOX_BYTES, tmB, n0 + 64, brow, bar);
-          brow += GG_BK;
+          r += GG_BK, brow += GG_BK;
           if (ROWS && brow == a.kb_rows) brow = 0;
+          if (!ROWS && --left == 0) left = once, r = brow = w.beg, acol += a.kpart_cols;
           if (++s == GG_STAGES) s = 0, ph ^= 1;
         }
       }
@@ -264,15 +269,16 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const Item w = fixed(nx);
       if (t + pairs < items) nx = item_of(t + pairs);
       const bool tail = tail_rows(w) != 0;
-      const int step = piece(w);
-      for (int beg = w.beg; beg < w.end && ok; beg += step, ++n) {
-        const int end = min(beg + step, w.end);
+      const int once = steps_once(w), steps = once * a.kparts, per = piece(steps);
+      int r = w.beg;
+      for (int i0 = 0; i0 < steps && ok; i0 += per, ++n) {
+        const int i1 = min(i0 + per, steps);
         const uint32_t buf = n & 1, d = tmem_base + buf * 256;
         if (!gg_wait(smem_u32(&sh->tmem_empty[buf]), ((n >> 1) & 1) ^ 1, abort_flag)) {
           ok = false;
           break;
         }
-        for (int r = beg; r < end; r += GG_BK) {
+        for (int i = i0; i < i1; ++i) {
           if (!gg_wait(smem_u32(&sh->full[0]) + s * 8, ph, abort_flag)) {
             ok = false;
             break;
@@ -283,13 +289,15 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (lane == 0) {
             tc_fence_after();
             const uint64_t adesc = adesc0 + (uint64_t)(s * (GG_STAGE_BYTES >> 4)), bdesc = bdesc0 + (uint64_t)(s * (GG_STAGE_BYTES >> 4));
-            const int rows = end - r;
+            const int rows = w.end - r;
 #pragma unroll
             for (int k16 = 0; k16 < GG_BK / 16; ++k16)  // +16 rows of 128 B (MN-major) or +32 B inside the swizzle atom (K-major)
               if (k16 * 16 < rows)
-                gg_mma(d, adesc + (uint64_t)(k16 * (ROWS ? 2 : 128)), bdesc + (uint64_t)(k16 * 128), idesc, (r > beg || k16 > 0) ? 1u : 0u);
+                gg_mma(d, adesc + (uint64_t)(k16 * (ROWS ? 2 : 128)), bdesc + (uint64_t)(k16 * 128), idesc, (i > i0 || k16 > 0) ? 1u : 0u);
             gg_commit(smem_u32(&sh->empty[0]) + s * 8);
           }
+          r += GG_BK;
+          if (r >= w.end) r = w.beg;
           if (++s == GG_STAGES) s = 0, ph ^= 1;
         }
         if (ok && lane == 0) gg_commit(smem_u32(&sh->tmem_full[buf]));
@@ -305,7 +313,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     for (int t = pair0; t < items; t += pairs) {
       const Item w = fixed(nx);
       if (t + pairs < items) nx = item_of(t + pairs);
-      at += (uint32_t)(max(w.end - w.beg, 0) + GG_BK - 1) / GG_BK;
+      at += (uint32_t)(steps_once(w) * a.kparts);
       const int rows = w.beg < w.end ? tail_rows(w) : 0;
       if (!rows) continue;
       const uint32_t s = (at - 1) % GG_STAGES;
@@ -378,7 +386,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         continue;
       }
       auto put = [&](uint4* p, int i, uint4 v) { p[lane * 8 + (i ^ (lane & 7))] = v; };  // the 128-byte swizzle
-      const int step = piece(w);
+      const int steps = steps_once(w) * a.kparts, per = piece(steps);
       auto release = [&](uint32_t buf) {  // the accumulator is in registers (or nobody wants it)
         tc_fence_before();
         __syncwarp();
@@ -388,7 +396,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         float acc[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-        for (int beg = w.beg; beg < w.end; beg += step, ++n) {
+        for (int i0 = 0; i0 < steps; i0 += per, ++n) {
           const uint32_t buf = n & 1;
           if (!gg_wait(smem_u32(&sh->tmem_full[buf]), (n >> 1) & 1, abort_flag)) {
             ok = false;
@@ -533,7 +541,8 @@ int gg_launch(const CUtensorMap (&tm)[6], const GgArgs& a, cudaStream_t st) {
 
 int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   CUtensorMap tm[6];
-  const int64_t acols = (int64_t)g.segs * g.M;
+  if (g.kparts > 1 && (g.segs > 1 || g.offsets)) return B200MOE_EINVAL;  // (their ends are ends of the tensor or of whole steps)
+  const int64_t acols = (int64_t)g.segs * g.M * g.kparts;
   if (!gg_make_map(&tm[0], g.a, false, (uint64_t)g.P, (uint64_t)acols, GG_BK)) return B200MOE_EDRIVER;
   if (!gg_make_map(&tm[1], g.b0, false, (uint64_t)g.P, (uint64_t)g.N, GG_BK)) return B200MOE_EDRIVER;
   if (!gg_make_map(&tm[2], g.b1 ? g.b1 : g.b0, false, (uint64_t)g.P, (uint64_t)g.N, GG_BK)) return B200MOE_EDRIVER;
@@ -546,6 +555,7 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   a.M = g.M, a.N = g.N;
   a.MT = (g.M + 255) / 256, a.NT = (g.N + 255) / 256;
   a.out_rows = g.M;
+  a.kparts = g.kparts, a.kpart_cols = g.M;
   a.out0 = reinterpret_cast<uint8_t*>(g.out[0]), a.out1 = reinterpret_cast<uint8_t*>(g.out[1]), a.out2 = reinterpret_cast<uint8_t*>(g.out[2]);
   a.add = g.add;
   a.status = g.status;
@@ -563,6 +573,7 @@ int moe_row_product_tc(__nv_bfloat16* out, const __nv_bfloat16* a16, int lda, co
   a.groups = a.segs = 1;
   a.M = (int)rows, a.N = N;
   a.MT = (int)((rows + 255) / 256), a.NT = (N + 255) / 256;
+  a.kparts = 1;
   a.K = K, a.kb_rows = b_cycle;
   a.status = status;
   return gg_launch<true, false>(tm, a, st);

@@ -809,22 +809,30 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
               }
               wst[lane * 4 + (v4 ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
             }
+            // (d has been read: its place takes the 32 rows x 128 bytes of bf16)
+            uint4* wst16 = reinterpret_cast<uint4*>(smem + (size_t)TC_GRAD_STAGES * TC_STAGE_BYTES + wepi * 6144);
+            if (g16) {
+#pragma unroll
+              for (int v4 = 0; v4 < 8; ++v4) {
+                uint32_t ow[4];
+#pragma unroll
+                for (int w4 = 0; w4 < 4; ++w4) {
+                  const float2 v = unpack2(acc[m][v4 * 4 + w4]);
+                  ow[w4] = pack_bf16(v.x, v.y);
+                }
+                wst16[lane * 8 + (v4 ^ (lane & 7))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+              }
+            }
             store_patch(a.hq, (int64_t)a.I * 2, (int64_t)m * a.I + col);
             if (g16) {
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                for (int v4 = 0; v4 < 4; ++v4) {
-                  uint32_t ow[4];
-#pragma unroll
-                  for (int w4 = 0; w4 < 4; ++w4) {
-                    const float2 v = unpack2(acc[m][half * 16 + v4 * 4 + w4]);
-                    ow[w4] = pack_bf16(v.x, v.y);
-                  }
-                  wst[lane * 4 + (v4 ^ ((lane >> 1) & 3))] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
-                }
-                store_patch(g16, g16_stride, (int64_t)m * a.I * 2 + (col + half * 32) * 2);
+              for (int i = 0; i < 8; ++i) {  // 4 rows x 128 B per instruction
+                const int r = i * 4 + (lane >> 3), c = lane & 7;
+                const int orow = row0 + q * 32 + r;
+                if (orow < row_end)
+                  *reinterpret_cast<uint4*>(g16 + orow * g16_stride + (int64_t)m * a.I * 2 + col * 2 + c * 16) = wst16[r * 8 + (c ^ (r & 7))];
               }
+              __syncwarp();
             }
           }
         }

@@ -198,7 +198,6 @@ struct PrepArgs {
   const int32_t* pos_of;
   int64_t ld;
   int H, warps_per_row;
-  float* acc32;              // fp32 [side 0's rows, H] cleared on the way, or NULL
   MoeIdentityLists lists;    // written for side 0's rows (offsets NULL = none)
 };
 __global__ void __launch_bounds__(256)
@@ -215,10 +214,7 @@ grad_prep_kernel(const PrepArgs a) {
   uint4 raw[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) raw[i] = in ? *reinterpret_cast<const uint4*>(sd.src + r * H + c + i * 8) : make_uint4(0, 0, 0, 0);
-  if (a.acc32 && blockIdx.y == 0 && in) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(a.acc32 + r * H + c)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
+  int32_t my_pos = a.pos_of && lane < sd.slots ? a.pos_of[r * sd.slots + lane] : -1;  // the slots' positions, one per lane
   float v[16], amax = 0.f;
   const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(raw);
 #pragma unroll
@@ -237,7 +233,8 @@ grad_prep_kernel(const PrepArgs a) {
   out.z = moe_f32x4_to_e4m3x4(v[8] * inv, v[9] * inv, v[10] * inv, v[11] * inv);
   out.w = moe_f32x4_to_e4m3x4(v[12] * inv, v[13] * inv, v[14] * inv, v[15] * inv);
   for (int j = 0; j < sd.slots; ++j) {
-    const int64_t p = a.pos_of ? a.pos_of[r * sd.slots + j] : r;
+    if (a.pos_of && j > 0 && (j & 31) == 0) my_pos = j + lane < sd.slots ? a.pos_of[r * sd.slots + j + lane] : -1;
+    const int64_t p = a.pos_of ? __shfl_sync(0xffffffffu, my_pos, j & 31) : r;
     if (p < 0 || !in) continue;
     *reinterpret_cast<uint4*>(sd.q + p * H + c) = out;
     if ((lane & 7) == 0) sd.s_t[(int64_t)(c >> 7) * a.ld + p] = sc;
@@ -367,9 +364,10 @@ split_logits_kernel(__nv_bfloat16* split, const float* dlogits, int64_t T, int E
 #pragma unroll
   for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(split + (t * 3 + i) * Ep + e0) = *reinterpret_cast<const uint2*>(o[i]);
 }
-// dwr[e,h] (+)= sum over the parts, in order, of part[i][e,h] + (part[i][Ep+e,h] + part[i][2Ep+e,h])
+// dwr[e,h] (+)= sum over the parts, in order, of part[i][e,h] + (part[i][Ep+e,h] + part[i][2Ep+e,h]); a part has 3 Ep rows, or Ep
+// where the three were summed already
 __global__ void __launch_bounds__(256)
-router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int E, int Ep, int H) {
+router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int rows, int E, int Ep, int H) {
   pdl_begin();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int hv = H / 4;
@@ -378,9 +376,10 @@ router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int
   const int c = (int)(i - e * hv) * 4;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < parts; ++s) {
-    const float* p = part + ((int64_t)s * 3 * Ep + e) * H + c;
-    const float4 v0 = *reinterpret_cast<const float4*>(p), v1 = *reinterpret_cast<const float4*>(p + (int64_t)Ep * H),
-                 v2 = *reinterpret_cast<const float4*>(p + (int64_t)2 * Ep * H);
+    const float* p = part + ((int64_t)s * rows + e) * H + c;
+    const float4 v0 = *reinterpret_cast<const float4*>(p);
+    float4 v1 = make_float4(0.f, 0.f, 0.f, 0.f), v2 = v1;
+    if (rows > Ep) v1 = *reinterpret_cast<const float4*>(p + (int64_t)Ep * H), v2 = *reinterpret_cast<const float4*>(p + (int64_t)2 * Ep * H);
     acc[0] += v0.x + (v1.x + v2.x), acc[1] += v0.y + (v1.y + v2.y), acc[2] += v0.z + (v1.z + v2.z), acc[3] += v0.w + (v1.w + v2.w);
   }
   if (f32) {
@@ -486,22 +485,25 @@ extern "C" int b200moe_combine_backward(void* dy, float* dw, const void* dout, c
 namespace {
 struct RouterLayout {
   size_t split, part, total;
-  int Ep, parts;
+  int Ep, parts, stacked;  // stacked: dlogits' three numbers as one K range, else as rows of output
 };
 RouterLayout router_layout(int64_t T, int64_t H, int64_t E) {
   RouterLayout L{};
   Carve w;
   L.Ep = (int)align_up((size_t)E, 64);
-  // A tile is 256 x 256 outputs and 74 CTA pairs work at a time.  The tokens are cut into parts so that the rounds of
-  // (tile, part) items come out short: K steps of an item, plus four for what an item costs at its end and in the sum of the parts.
+  // A tile is 256 x 256 outputs and 74 CTA pairs work at a time.  dlogits' three numbers are three times the output rows,
+  // or three times the K range where that is no more tiles' work (256 experts: a third of the partial sums).  The tokens
+  // are cut into parts so that the rounds of (tile, part) items come out short: K steps of an item, plus four for what an item
+  // costs at its end and in the sum of the parts.
   // (The sizes alone decide, not the device: a workspace fits wherever it was sized.)
-  const int64_t tiles = (3 * L.Ep + 255) / 256 * ((H + 255) / 256), steps = (T + 63) / 64;
+  const int64_t nt = (H + 255) / 256, steps = (T + 63) / 64;
   int64_t best = 0;
-  L.parts = 1;
-  for (int64_t p = 1; p <= 16 && p * 2 <= std::max<int64_t>(steps, 2); ++p) {
-    const int64_t cost = (tiles * p + 73) / 74 * ((steps + p - 1) / p + 4);
-    if (p == 1 || cost < best) best = cost, L.parts = (int)p;
-  }
+  for (int64_t p = 1; p <= 16 && p * 2 <= std::max<int64_t>(steps, 2); ++p)
+    for (int st = 0; st < 2; ++st) {
+      const int64_t tiles = ((st ? 1 : 3) * L.Ep + 255) / 256 * nt;
+      const int64_t cost = (tiles * p + 73) / 74 * ((steps + p - 1) / p * (st ? 3 : 1) + 4);
+      if (best == 0 || cost < best) best = cost, L.parts = (int)p, L.stacked = st;
+    }
   L.split = w.take((size_t)T * 3 * L.Ep * 2);
   L.part = w.take((size_t)std::min<int64_t>(16, std::max<int64_t>(steps / 2, 1)) * 3 * L.Ep * H * 4);  // (for any number of parts: never smaller for more tokens)
   L.total = w.total;
@@ -552,13 +554,13 @@ extern "C" int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype
     g.b0 = reinterpret_cast<const __nv_bfloat16*>(x);
     g.out[0] = part;
     g.P = T;
-    g.groups = L.parts, g.segs = 1, g.M = 3 * L.Ep, g.N = (int)H;
+    g.groups = L.parts, g.segs = 1, g.kparts = L.stacked ? 3 : 1, g.M = (L.stacked ? 1 : 3) * L.Ep, g.N = (int)H;
     g.out_f32 = 1;
     g.status = status;
     rc = moe_weight_grad_tc(g, st);
     if (!rc)
       rc = moe_launch(router_dwr_kernel, (unsigned)((E * (H / 4) + 255) / 256), 256, 0, st, dwr, (int)(dwr_dtype == B200MOE_F32),
-                      accumulate, part, L.parts, (int)E, L.Ep, (int)H);
+                      accumulate, part, L.parts, g.M, (int)E, L.Ep, (int)H);
   }
   if (!rc && dx)
     rc = moe_row_product_tc(reinterpret_cast<__nv_bfloat16*>(dx), split, 3 * L.Ep, reinterpret_cast<const __nv_bfloat16*>(wr), T,
@@ -662,7 +664,7 @@ extern "C" int b200moe_linear_w8_backward(void* dx, void* dw, int dw_dtype, int 
     g.b0 = reinterpret_cast<const __nv_bfloat16*>(x);
     g.out[0] = dw;
     g.P = M;
-    g.groups = g.segs = 1, g.M = (int)N, g.N = (int)K;
+    g.groups = g.segs = g.kparts = 1, g.M = (int)N, g.N = (int)K;
     g.out_f32 = dw_dtype == B200MOE_F32, g.add = accumulate;
     g.status = status;
     rc = moe_weight_grad_tc(g, st);
@@ -787,7 +789,6 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
   p.pos_of = I32(L.pos_of);
   p.ld = L.ld;
   p.H = (int)d->H;
-  p.acc32 = nullptr;
   rc = launch_prep(p, st);
   if (rc) return rc;
 
@@ -858,7 +859,7 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
     wg.out[0] = dw_gate, wg.out[1] = dw_up, wg.out[2] = dw_down;
     wg.offsets = I32(L.offsets);
     wg.P = L.P;
-    wg.groups = (int)d->E, wg.segs = 3, wg.M = (int)d->I, wg.N = (int)d->H;
+    wg.groups = (int)d->E, wg.segs = 3, wg.kparts = 1, wg.M = (int)d->I, wg.N = (int)d->H;
     wg.out_f32 = d->grad_dtype == B200MOE_F32, wg.add = d->accumulate;
     wg.status = status;
     rc = moe_weight_grad_tc(wg, st);
