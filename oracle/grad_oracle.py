@@ -41,7 +41,8 @@ def quant_rows(v, floor):
     return cut(q * s), cut(step * s), cut(away * s)
 
 
-def route_backward(dw, logits, ids, score, renorm, scale, logit_bias=None):
+def route_backward(dw, logits, ids, score, renorm, scale, logit_bias=None, dw_bound=None):
+    """``dw_bound``: how far dw itself may be from what is given here; the result's bound then covers that too."""
     T, E = logits.shape
     l = logits.double() + (logit_bias.double() if logit_bias is not None else 0.0)
     p = torch.softmax(l, -1) if score == "softmax" else torch.sigmoid(l)
@@ -51,20 +52,23 @@ def route_backward(dw, logits, ids, score, renorm, scale, logit_bias=None):
     d = dw.double() * on
     S = pj.sum(-1, keepdim=True)
     dp = scale * (d - (d * pj).sum(-1, keepdim=True) / S) / S if renorm else scale * d
-    size = scale * (d.abs() + (d.abs() * pj).sum(-1, keepdim=True) / S) / S if renorm else scale * d.abs()
-    dp, size = dp * on, size * on
+    dp = dp * on
     dense = torch.zeros_like(l).scatter_add_(1, safe, dp)
-    dense_size = torch.zeros_like(l).scatter_add_(1, safe, size)
-    if score == "softmax":
-        mean, mean_size = (dp * pj).sum(-1, keepdim=True), (size * pj).sum(-1, keepdim=True)
-        if renorm:
-            mean, mean_size = torch.zeros_like(mean), torch.zeros_like(mean)
-        out, big = p * (dense - mean), p * (dense_size + mean_size)
-    else:
-        out, big = dense * p * (1 - p), dense_size * p * (1 - p)
+    slope = p if score == "softmax" else p * (1 - p)
+    mean = (dp * pj).sum(-1, keepdim=True) if score == "softmax" and not renorm else 0.0
+    out = slope * (dense - mean)
+
+    def reach(e):  # the same sums over the sizes of what goes into them
+        size = scale * (e + (e * pj).sum(-1, keepdim=True) / S) / S if renorm else scale * e
+        size = size * on
+        spread = (size * pj).sum(-1, keepdim=True) if score == "softmax" and not renorm else 0.0
+        return slope * (torch.zeros_like(l).scatter_add_(1, safe, size) + spread)
+
+    big = reach(d.abs())
     # a few operations with k-fold and E-fold sums; expf is good to 2 steps and its argument l - m to one step of |l|
     k = ids.shape[1]
-    return out, big * U * (2 * k + 40 + 4 * l[torch.isfinite(l)].abs().max() + E / 16)
+    bound = big * U * (2 * k + 40 + 4 * l[torch.isfinite(l)].abs().max() + E / 16)
+    return out, bound if dw_bound is None else bound + reach(dw_bound.double() * on)
 
 
 def combine_backward(dout, y, w, ids=None, E=0):

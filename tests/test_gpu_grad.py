@@ -163,7 +163,7 @@ def test_combine_backward_masked_and_in_place(ops):
 
 # ---- router product --------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("T,H,E", [(1, 8, 1), (1, 1024, 8), (16, 1000, 8), (65, 264, 64), (130, 128, 65), (257, 2048, 128), (300, 520, 300),
-                                   (63, 256, 1024), (1500, 776, 8), (4500, 264, 16)])
+                                   (63, 256, 1024), (1500, 776, 8), (4500, 264, 16), (700, 7168, 256), (64, 136, 128), (65, 136, 128)])
 def test_router_logits_backward(ops, T, H, E):
     g = gen(T + H + E)
     dl, x, wr = randn(g, T, E, dtype=torch.float32), randn(g, T, H), randn(g, E, H, scale=0.1)
@@ -180,6 +180,10 @@ def test_router_logits_backward(ops, T, H, E):
     base = randn(g, E, H, dtype=torch.float32)
     acc = ops.router_logits_backward(dl, x, None, dwr=base.clone(), accumulate=True)[1]
     assert torch.equal(acc, base + dwr)
+    into = randn(g, T, H)
+    got = ops.router_logits_backward(dl, None, wr, dx=into.clone(), add_dx=True)[0]
+    want = into.double() + wx
+    within(got, want, rounded(want, bx + (wx.abs() + bx) * G.half_step(torch.bfloat16), torch.bfloat16), "added to dx")
     assert int(st.item()) == 0
 
 

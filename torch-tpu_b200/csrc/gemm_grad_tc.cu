@@ -70,7 +70,7 @@ struct GgArgs {
   int kparts, kpart_cols;  // the K range is walked kparts times, with columns of A kpart_cols further each time
   int K;                   // row product: depth; B's row of step k is k % kb_rows
   int kb_rows;
-  int add;                 // results are added to the output (fp32)
+  int add;                 // results are added to the output
   uint8_t *out0, *out1, *out2;  // the segments' outputs, for groups without rows
   int32_t* status;
 };
@@ -482,8 +482,8 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           patches_written();
           if (lane == 0) {
-            gg_store(map, col0, row, smem_u32(p), false);
-            if (PER < cols) gg_store(map, col0 + PER, row, smem_u32(p) + GG_PATCH_BYTES, false);
+            gg_store(map, col0, row, smem_u32(p), a.add);
+            if (PER < cols) gg_store(map, col0 + PER, row, smem_u32(p) + GG_PATCH_BYTES, a.add);
             sent();
           }
         }
@@ -562,7 +562,7 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   return g.out_f32 ? gg_launch<false, true>(tm, a, st) : gg_launch<false, false>(tm, a, st);
 }
 
-int moe_row_product_tc(__nv_bfloat16* out, const __nv_bfloat16* a16, int lda, const __nv_bfloat16* b, int64_t rows, int K, int b_rows,
+int moe_row_product_tc(__nv_bfloat16* out, bool add, const __nv_bfloat16* a16, int lda, const __nv_bfloat16* b, int64_t rows, int K, int b_rows,
                        int b_cycle, int N, int32_t* status, cudaStream_t st) {
   CUtensorMap tm[6];
   if (!gg_make_map(&tm[0], a16, false, (uint64_t)rows, (uint64_t)K, 128, (uint64_t)lda)) return B200MOE_EDRIVER;
@@ -574,6 +574,7 @@ int moe_row_product_tc(__nv_bfloat16* out, const __nv_bfloat16* a16, int lda, co
   a.M = (int)rows, a.N = N;
   a.MT = (int)((rows + 255) / 256), a.NT = (N + 255) / 256;
   a.kparts = 1;
+  a.add = add;
   a.K = K, a.kb_rows = b_cycle;
   a.status = status;
   return gg_launch<true, false>(tm, a, st);

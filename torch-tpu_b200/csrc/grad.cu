@@ -398,7 +398,7 @@ router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int
 constexpr int RGS_COLS = 32, RGS_THREADS = 256, RGS_ROWS = RGS_THREADS / RGS_COLS;
 constexpr int RGS_MAX_T = 64, RGS_MAX_TE = 8192;  // tokens, tokens x experts
 __global__ void __launch_bounds__(RGS_THREADS)
-router_small_grad_kernel(__nv_bfloat16* dx, void* dwr, int f32, int add, const float* dlogits, const __nv_bfloat16* x,
+router_small_grad_kernel(__nv_bfloat16* dx, int add_dx, void* dwr, int f32, int add, const float* dlogits, const __nv_bfloat16* x,
                          const __nv_bfloat16* wr, int T, int H, int E) {
   pdl_begin();
   extern __shared__ float rgs[];
@@ -416,7 +416,8 @@ router_small_grad_kernel(__nv_bfloat16* dx, void* dwr, int f32, int add, const f
       float s = 0.f;
 #pragma unroll 8
       for (int e = 0; e < E; ++e) s = fmaf(dl[t * E + e], ws[e * RGS_COLS + c], s);
-      dx[(int64_t)t * H + h] = __float2bfloat16_rn(s);
+      __nv_bfloat16* o = dx + (int64_t)t * H + h;
+      *o = __float2bfloat16_rn(add_dx ? s + __bfloat162float(*o) : s);
     }
   if (x)
     for (int e = r; e < E; e += RGS_ROWS) {
@@ -516,15 +517,15 @@ extern "C" size_t b200moe_router_logits_backward_workspace_bytes(int64_t T, int6
   return router_layout(T, H, E).total;
 }
 
-extern "C" int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype, int accumulate, const float* dlogits, const void* x,
-                                              const void* wr, int64_t T, int64_t H, int64_t E, void* workspace,
+extern "C" int b200moe_router_logits_backward(void* dx, int add_dx, void* dwr, int dwr_dtype, int accumulate, const float* dlogits,
+                                              const void* x, const void* wr, int64_t T, int64_t H, int64_t E, void* workspace,
                                               size_t workspace_bytes, int32_t* status, void* stream) {
-  MOE_CHECK_ARG(T >= 0 && H > 0 && E > 0 && (dx || dwr));
+  MOE_CHECK_ARG(T >= 0 && H > 0 && E > 0 && (add_dx == 0 || add_dx == 1));
   MOE_CHECK_ARG(!dwr || grad_dtype_ok(dwr_dtype, accumulate));
   MOE_CHECK_SHAPE(H % 8 == 0 && E <= 1024 && T < (1 << 24) && H < (1 << 24));
   cudaStream_t st = (cudaStream_t)stream;
   if (T == 0) return zero_grad(dwr, (size_t)E * H * grad_elem(dwr_dtype), accumulate, st);
-  MOE_CHECK_ARG(dlogits && (!dx || wr) && (!dwr || x));
+  MOE_CHECK_ARG(dlogits && (dx || dwr) && (!dx || wr) && (!dwr || x) && (!add_dx || dx));
   if ((dx && !(moe_aligned16(dx) && moe_aligned16(wr))) || (dwr && !(moe_aligned16(dwr) && moe_aligned16(x)))) return B200MOE_EALIGN;
   if (!moe_tc_available()) return B200MOE_EDRIVER;
   const RouterLayout L = router_layout(T, H, E);
@@ -539,7 +540,7 @@ extern "C" int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype
       attr_set[dev] = true;
     }
     return moe_launch(router_small_grad_kernel, (unsigned)((H + RGS_COLS - 1) / RGS_COLS), RGS_THREADS, smem, st,
-                      reinterpret_cast<__nv_bfloat16*>(dx), dwr, (int)(dwr_dtype == B200MOE_F32), accumulate, dlogits,
+                      reinterpret_cast<__nv_bfloat16*>(dx), add_dx, dwr, (int)(dwr_dtype == B200MOE_F32), accumulate, dlogits,
                       reinterpret_cast<const __nv_bfloat16*>(dwr ? x : nullptr), reinterpret_cast<const __nv_bfloat16*>(wr), (int)T, (int)H,
                       (int)E);
   }
@@ -563,7 +564,7 @@ extern "C" int b200moe_router_logits_backward(void* dx, void* dwr, int dwr_dtype
                       accumulate, part, L.parts, g.M, (int)E, L.Ep, (int)H);
   }
   if (!rc && dx)
-    rc = moe_row_product_tc(reinterpret_cast<__nv_bfloat16*>(dx), split, 3 * L.Ep, reinterpret_cast<const __nv_bfloat16*>(wr), T,
+    rc = moe_row_product_tc(reinterpret_cast<__nv_bfloat16*>(dx), add_dx != 0, split, 3 * L.Ep, reinterpret_cast<const __nv_bfloat16*>(wr), T,
                             2 * L.Ep, (int)E, L.Ep, (int)H, status, st);
   return rc;
 }
@@ -602,13 +603,13 @@ extern "C" size_t b200moe_linear_w8_backward_workspace_bytes(int64_t M, int64_t 
 extern "C" int b200moe_linear_w8_backward(void* dx, void* dw, int dw_dtype, int accumulate, const void* dy, const void* x,
                                           const void* w, const void* scale, int scale_dtype, int64_t M, int64_t K, int64_t N,
                                           void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-  MOE_CHECK_ARG(M >= 0 && K > 0 && N > 0 && (dx || dw));
+  MOE_CHECK_ARG(M >= 0 && K > 0 && N > 0);
   MOE_CHECK_ARG(!dw || grad_dtype_ok(dw_dtype, accumulate));
   MOE_CHECK_ARG(scale_dtype == B200MOE_F32 || scale_dtype == B200MOE_BF16);
   MOE_CHECK_SHAPE(K % kBlock == 0 && N % 64 == 0 && M < (1 << 24) && K < (1 << 24) && N < (1 << 24));
   cudaStream_t st = (cudaStream_t)stream;
   if (M == 0) return zero_grad(dw, (size_t)N * K * grad_elem(dw_dtype), accumulate, st);
-  MOE_CHECK_ARG(dy && (!dx || (w && scale)) && (!dw || x));
+  MOE_CHECK_ARG(dy && (dx || dw) && (!dx || (w && scale)) && (!dw || x));
   if (!moe_aligned16(dy) || (dx && !(moe_aligned16(dx) && moe_aligned16(w))) || (dw && !(moe_aligned16(dw) && moe_aligned16(x))))
     return B200MOE_EALIGN;
   if (!moe_tc_available()) return B200MOE_EDRIVER;
@@ -743,7 +744,6 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const bool wgrad = d->weight_grads;
-  MOE_CHECK_ARG(dx || dw || wgrad);
   if (wgrad) MOE_CHECK_ARG(dw_gate && dw_up && dw_down);
   if (d->T == 0) {
     if (wgrad)
@@ -753,6 +753,7 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
       }
     return B200MOE_OK;
   }
+  MOE_CHECK_ARG(dx || dw || wgrad);  // (empty tensors may carry null pointers)
   MOE_CHECK_ARG(dout && x && w_gate && w_up && w_down && s_gate && s_up && s_down && ids);
   MOE_CHECK_ARG(d->per_slot ? !topk_w && !dw : topk_w != nullptr);
   MOE_CHECK_ARG(!add || dx);

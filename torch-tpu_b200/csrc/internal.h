@@ -151,7 +151,8 @@ struct MoeWeightGradArgs {
 };
 int moe_weight_grad_tc(const MoeWeightGradArgs& a, cudaStream_t st);
 // out[r, :N] = sum over k < K of a[r * lda + k] * b[k % b_cycle, :N], b [b_rows, N] (rows past b_rows count as zeros); K, b_cycle % 64 == 0
-int moe_row_product_tc(__nv_bfloat16* out, const __nv_bfloat16* a, int lda, const __nv_bfloat16* b, int64_t rows, int K, int b_rows,
+// (add: to what out holds)
+int moe_row_product_tc(__nv_bfloat16* out, bool add, const __nv_bfloat16* a, int lda, const __nv_bfloat16* b, int64_t rows, int K, int b_rows,
                        int b_cycle, int N, int32_t* status, cudaStream_t st);
 int moe_f32_rows_to_bf16(__nv_bfloat16* out, const float* in, int64_t n, cudaStream_t st);
 int moe_device_sm_count();

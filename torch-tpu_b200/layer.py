@@ -25,6 +25,16 @@ class MoEConfig:
     shared_intermediate: int = 0     # 0 = no shared expert
 
 
+@dataclass
+class MoEGrads:
+    """What FusedMoE.backward returns; None = not asked for."""
+    dx: torch.Tensor                 # bf16 [T,H]
+    dlogits: torch.Tensor            # fp32 [T,E] (summed over the tokens: the gradient of logit_bias)
+    router: Optional[torch.Tensor]   # [E,H]
+    experts: Optional[Tuple]         # (dwg, dwu, dwd), [E,I,H] each
+    shared: Optional[Tuple]
+
+
 class FusedMoE:
     """One MoE layer on one GPU.  Weights are in the op layout: gate/up/down ``[E,I,H]`` float8_e4m3fn (down =
     W_down^T contiguous), scales ``[E,I/128,H/128]`` fp32 or bf16, router ``[E,H]`` bf16, optional selection bias
@@ -50,6 +60,7 @@ class FusedMoE:
         self.x_dev = torch.empty(max_tokens, H, dtype=torch.bfloat16, device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._graphs = {}
+        self._bwd = {}   # buffers of backward(), made by its first call
         self.workspace = None
         if alloc_workspace:  # an expert-parallel shard runs its experts through other entry points
             d = ops.make_desc(max_tokens, H, cfg.intermediate, E, k, I_shared=cfg.shared_intermediate,
@@ -77,6 +88,57 @@ class FusedMoE:
                            fused_combine=self.fused_combine)
 
     __call__ = forward
+
+    def backward(self, x, dout, *, router_grad=None, weight_grads=None, shared_grads=None, accumulate=False, dx=None):
+        """Gradients of ``forward(x)`` for dout = d(loss)/d(out), bf16 [T,H]: the routing, gate and up are formed again from x
+        (nothing of the forward call is kept, so calls need not alternate).  Returns ``MoEGrads``.
+
+        ``router_grad`` [E,H] fp32 or bf16, ``weight_grads`` = (dwg, dwu, dwd) [E,I,H] and ``shared_grads`` (the same for the
+        shared expert, leading dim 1) are buffers that receive the weights' gradients; what is None is not formed.
+        ``accumulate`` adds to what they hold (fp32).  Views of internal buffers are returned, unless ``dx`` is given, and
+        hold until the next call.  Allocates on the first call of a kind only; can be captured into a CUDA graph after it.
+        FP8 weights and W8A8 arithmetic only.  Not an autograd function: the caller chains it, last layer first."""
+        T, H = x.shape
+        c = self.cfg
+        if T > self.max_tokens:
+            raise ValueError(f"{T} tokens > max_tokens={self.max_tokens}")
+        if self.act_mode != L.ACT_W8A8 or self.w[0].dtype != torch.float8_e4m3fn:
+            raise ValueError("the gradient is that of FP8 weights in W8A8 arithmetic")
+        if shared_grads is not None and self.shared is None:
+            raise ValueError("shared_grads without a shared expert")
+        b = self._backward_buffers(weight_grads is not None, shared_grads is not None)
+        ids, w = self.route(x) if T else (self.ids[:0], self.topk_w[:0])
+        dx = b["dx"][:T] if dx is None else dx
+        if self.shared is not None:  # the shared expert is one expert that every token takes with weight 1
+            ops.experts_backward(dout, x, *self.shared, b["zeros"][:T], b["ones"][:T], dx=dx, dw=b["shared_dw"][:T],
+                                 weight_grads=shared_grads, accumulate=accumulate, workspace=b["workspace"], status=self.status)
+        _, dw = ops.experts_backward(dout, x, *self.w, ids, w, dx=dx, dw=b["dw"][:T], add=dx if self.shared is not None else None,
+                                     weight_grads=weight_grads, accumulate=accumulate, workspace=b["workspace"], status=self.status)
+        dlogits = ops.route_backward(dw, self.logits[:T], ids, c.score_func, c.renorm, c.routed_scale, self.logit_bias,
+                                     dlogits=b["dlogits"][:T])
+        ops.router_logits_backward(dlogits, x if router_grad is not None else None, self.router_w, dx=dx, dwr=router_grad,
+                                   accumulate=accumulate and router_grad is not None, add_dx=True, workspace=b["workspace"], status=self.status)
+        return MoEGrads(dx, dlogits, router_grad, weight_grads, shared_grads)
+
+    def _backward_buffers(self, weight_grads, shared_grads):
+        b = self._bwd
+        c, n, dev = self.cfg, self.max_tokens, self.device
+        need = [ops.experts_backward_workspace_bytes(ops.make_backward_desc(
+            n, c.hidden, c.intermediate, c.num_experts, c.top_k, scale_dtype=self.w[3].dtype, weight_grads=weight_grads)),
+            L.lib().b200moe_router_logits_backward_workspace_bytes(n, c.hidden, c.num_experts)]
+        if self.shared is not None:
+            need.append(ops.experts_backward_workspace_bytes(ops.make_backward_desc(
+                n, c.hidden, c.shared_intermediate, 1, 1, scale_dtype=self.shared[3].dtype, weight_grads=shared_grads)))
+        if not b:
+            b.update(dx=torch.empty(n, c.hidden, dtype=torch.bfloat16, device=dev),
+                     dw=torch.empty(n, c.top_k, dtype=torch.float32, device=dev),
+                     dlogits=torch.empty(n, c.num_experts, dtype=torch.float32, device=dev), workspace=None)
+            if self.shared is not None:
+                b.update(zeros=torch.zeros(n, 1, dtype=torch.int32, device=dev), ones=torch.ones(n, 1, device=dev),
+                         shared_dw=torch.empty(n, 1, dtype=torch.float32, device=dev))
+        if b["workspace"] is None or b["workspace"].numel() < max(need) + 256:
+            b["workspace"] = torch.empty(max(need) + 256, dtype=torch.uint8, device=dev)
+        return b
 
     def capture(self, T: int):
         """Capture forward() for exactly T tokens into a CUDA graph (the call allocates nothing and never touches the

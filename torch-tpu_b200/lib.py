@@ -79,7 +79,7 @@ SIGNATURES = {
                                   c_void_p, c_size_t, c_void_p, c_void_p]),
     "b200moe_route_backward": (c_int, [c_void_p] * 5 + [c_int, c_int64, c_int64, c_int64, c_int, c_int, c_float, c_void_p]),
     "b200moe_router_logits_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
-    "b200moe_router_logits_backward": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+    "b200moe_router_logits_backward": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                                c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
     "b200moe_combine_backward": (c_int, [c_void_p] * 5 + [c_int, c_void_p] + [c_int64] * 4 + [c_void_p]),
     "b200moe_linear_w8_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),

@@ -348,9 +348,11 @@ def route_backward(dw, logits, ids, score_func="softmax", renorm=True, scale=1.0
     return dlogits
 
 
-def router_logits_backward(dlogits, x=None, wr=None, dx=None, dwr=None, accumulate=False, workspace=None, status=None):
+def router_logits_backward(dlogits, x=None, wr=None, dx=None, dwr=None, accumulate=False, add_dx=False, workspace=None,
+                           status=None):
     """Gradients of ``router_logits``: (dx bf16 [T,H] = dlogits . wr, dwr [E,H] = dlogits^T . x).  Without ``wr`` dx is
-    None, without ``x`` dwr is.  ``dwr`` is fp32 unless a bf16 tensor is given; ``accumulate`` adds to what it holds (fp32)."""
+    None, without ``x`` dwr is.  ``dwr`` is fp32 unless a bf16 tensor is given; ``accumulate`` adds to what it holds (fp32).  ``add_dx`` adds to what ``dx`` holds (the
+    experts' dx, say)."""
     _rank(dlogits, "dlogits", 2)
     if x is None and wr is None:
         raise ValueError("x or wr is needed")
@@ -362,13 +364,15 @@ def router_logits_backward(dlogits, x=None, wr=None, dx=None, dwr=None, accumula
         _chk_accumulate(accumulate, dwr, "dwr")
     if wr is not None:
         _chk_grad(wr, "wr", _BF16, (E, H), dev)
+    if add_dx and (dx is None or wr is None):
+        raise ValueError("add_dx needs wr, and a dx to add to")
     _chk_status(status, dev)
     with _on(dev):
         need = L.lib().b200moe_router_logits_backward_workspace_bytes(T, H, E)
         keep, base, avail = _workspace(workspace, need, "b200moe_router_logits_backward", dev)
         dx = _grad_out(dx, "dx", _BF16, (T, H), dev) if wr is not None else None
         dwr = _grad_out(dwr, "dwr", _GRAD, (E, H), dev) if x is not None else None
-        L.check(L.lib().b200moe_router_logits_backward(_addr(dx), _addr(dwr), _DT[dwr.dtype] if dwr is not None else L.F32,
+        L.check(L.lib().b200moe_router_logits_backward(_addr(dx), int(add_dx), _addr(dwr), _DT[dwr.dtype] if dwr is not None else L.F32,
                                                        int(accumulate and dwr is not None), _addr(dlogits), _addr(x), _addr(wr), T, H, E,
                                                        base, avail, _addr(status), _raw_stream(dev)), "b200moe_router_logits_backward")
     return dx, dwr
