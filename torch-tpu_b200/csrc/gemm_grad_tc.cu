@@ -70,6 +70,7 @@ struct GgArgs {
   int kparts, kpart_cols;  // the K range is walked kparts times, with columns of A kpart_cols further each time
   int K;                   // row product: depth; B's row of step k is k % kb_rows
   int kb_rows;
+  int b_pairs;             // B's maps are of 64-column chunks (whole ones: N % 64 == 0)
   int add;                 // results are added to the output
   uint8_t *out0, *out1, *out2;  // the segments' outputs, for groups without rows
   int32_t* status;
@@ -98,6 +99,13 @@ __device__ __forceinline__ void gg_load(uint32_t dst, const CUtensorMap* map, in
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+// 128 columns of 64 rows, as two boxes of 64 columns behind each other (a map of 64-column chunks)
+__device__ __forceinline__ void gg_load_pair(uint32_t dst, const CUtensorMap* map, int chunk, int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(chunk), "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ uint32_t gg_in_cta(uint32_t addr, uint32_t rank) {
@@ -244,11 +252,14 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (ROWS) {
             gg_load(sa, &tmA, r, m0, bar);
           } else {
-            gg_load(sa, &tmA, acol, r, bar);
-            gg_load(sa + GG_BOX_BYTES, &tmA, acol + 64, r, bar);
+            gg_load_pair(sa, &tmA, acol / 64, r, bar);
           }
-          gg_load(sb, tmB, n0, brow, bar);
-          gg_load(sb + GG_BOX_BYTES, tmB, n0 + 64, brow, bar);
+          if (a.b_pairs) {
+            gg_load_pair(sb, tmB, n0 / 64, brow, bar);
+          } else {
+            gg_load(sb, tmB, n0, brow, bar);
+            gg_load(sb + GG_BOX_BYTES, tmB, n0 + 64, brow, bar);
+          }
           r += GG_BK, brow += GG_BK;
           if (ROWS && brow == a.kb_rows) brow = 0;
           if (!ROWS && --left == 0) left = once, r = brow = w.beg, acol += a.kpart_cols;
@@ -521,6 +532,23 @@ bool gg_make_map(CUtensorMap* m, const void* base, bool f32, uint64_t rows, uint
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// An MN-major operand (bf16 [rows, cols], cols % 64 == 0) as chunks of 64 columns: one copy brings 64 rows x 128 columns in the
+// layout that the MMAs read, where the plain map takes two (a copy costs its issuing thread over a hundred cycles: with four
+// per K step the producer was slower than the MMAs, 580 cycles a step against 512)
+bool gg_make_chunk_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {64, rows, cols / 64};
+  cuuint64_t strides[2] = {cols * 2, 128};
+  cuuint32_t box[3] = {64, GG_BK, 2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool gg_make_b_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols) {
+  return cols % 64 == 0 ? gg_make_chunk_map(m, base, rows, cols) : gg_make_map(m, base, false, rows, cols, GG_BK);
+}
+
 template <bool ROWS, bool F32>
 int gg_launch(const CUtensorMap (&tm)[6], const GgArgs& a, cudaStream_t st) {
   static bool attr_set[64] = {};
@@ -541,11 +569,12 @@ int gg_launch(const CUtensorMap (&tm)[6], const GgArgs& a, cudaStream_t st) {
 
 int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   CUtensorMap tm[6];
+  if (g.M % 64) return B200MOE_ESHAPE;
   if (g.kparts > 1 && (g.segs > 1 || g.offsets)) return B200MOE_EINVAL;  // (their ends are ends of the tensor or of whole steps)
   const int64_t acols = (int64_t)g.segs * g.M * g.kparts;
-  if (!gg_make_map(&tm[0], g.a, false, (uint64_t)g.P, (uint64_t)acols, GG_BK)) return B200MOE_EDRIVER;
-  if (!gg_make_map(&tm[1], g.b0, false, (uint64_t)g.P, (uint64_t)g.N, GG_BK)) return B200MOE_EDRIVER;
-  if (!gg_make_map(&tm[2], g.b1 ? g.b1 : g.b0, false, (uint64_t)g.P, (uint64_t)g.N, GG_BK)) return B200MOE_EDRIVER;
+  if (!gg_make_chunk_map(&tm[0], g.a, (uint64_t)g.P, (uint64_t)acols)) return B200MOE_EDRIVER;
+  if (!gg_make_b_map(&tm[1], g.b0, (uint64_t)g.P, (uint64_t)g.N)) return B200MOE_EDRIVER;
+  if (!gg_make_b_map(&tm[2], g.b1 ? g.b1 : g.b0, (uint64_t)g.P, (uint64_t)g.N)) return B200MOE_EDRIVER;
   for (int i = 0; i < 3; ++i)
     if (!gg_make_map(&tm[3 + i], g.out[i < g.segs ? i : 0], g.out_f32, (uint64_t)g.groups * g.M, (uint64_t)g.N, 32)) return B200MOE_EDRIVER;
   GgArgs a{};
@@ -558,6 +587,7 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   a.kparts = g.kparts, a.kpart_cols = g.M;
   a.out0 = reinterpret_cast<uint8_t*>(g.out[0]), a.out1 = reinterpret_cast<uint8_t*>(g.out[1]), a.out2 = reinterpret_cast<uint8_t*>(g.out[2]);
   a.add = g.add;
+  a.b_pairs = g.N % 64 == 0;
   a.status = g.status;
   return g.out_f32 ? gg_launch<false, true>(tm, a, st) : gg_launch<false, false>(tm, a, st);
 }
@@ -566,7 +596,7 @@ int moe_row_product_tc(__nv_bfloat16* out, bool add, const __nv_bfloat16* a16, i
                        int b_cycle, int N, int32_t* status, cudaStream_t st) {
   CUtensorMap tm[6];
   if (!gg_make_map(&tm[0], a16, false, (uint64_t)rows, (uint64_t)K, 128, (uint64_t)lda)) return B200MOE_EDRIVER;
-  if (!gg_make_map(&tm[1], b, false, (uint64_t)b_rows, (uint64_t)N, GG_BK)) return B200MOE_EDRIVER;
+  if (!gg_make_b_map(&tm[1], b, (uint64_t)b_rows, (uint64_t)N)) return B200MOE_EDRIVER;
   if (!gg_make_map(&tm[3], out, false, (uint64_t)rows, (uint64_t)N, 32)) return B200MOE_EDRIVER;
   tm[2] = tm[1], tm[4] = tm[5] = tm[3];
   GgArgs a{};
@@ -575,6 +605,7 @@ int moe_row_product_tc(__nv_bfloat16* out, bool add, const __nv_bfloat16* a16, i
   a.MT = (int)((rows + 255) / 256), a.NT = (N + 255) / 256;
   a.kparts = 1;
   a.add = add;
+  a.b_pairs = N % 64 == 0;
   a.K = K, a.kb_rows = b_cycle;
   a.status = status;
   return gg_launch<true, false>(tm, a, st);

@@ -138,7 +138,7 @@ int moe_gather_rows_bf16(__nv_bfloat16* dst, const __nv_bfloat16* x, const int32
 // weight gradients on the tensor cores (gemm_grad_tc.cu): out[seg][g * M + m, n] (+)= sum of a[r, seg * M + m] * b[r, n] over the
 // rows r of group g, b = b1 for segment 2, else b0.  Groups are [offsets[g], offsets[g+1]), clipped to P, or (offsets NULL) the
 // even parts of [0, P).  With kparts > 1 (one segment, no offsets) a has kparts * M columns and the sum is over those of every part
-// too.  M % 32 == 0, with several segments M % 128 == 0; N % 8 == 0
+// too.  M % 64 == 0, with several segments M % 128 == 0; N % 8 == 0
 struct MoeWeightGradArgs {
   const __nv_bfloat16* a;        // [P, segs * kparts * M]
   const __nv_bfloat16 *b0, *b1;  // [P, N]
