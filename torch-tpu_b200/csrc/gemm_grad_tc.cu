@@ -29,19 +29,29 @@
 #include <algorithm>
 
 #include "tc_ptx.cuh"
+#ifndef GGWIDE
+#define GGWIDE 1
+#endif
 
 namespace {
 
 constexpr int GG_EPI_WARPS = 8;
 constexpr int GG_THREADS = 128 + 32 * GG_EPI_WARPS;
-constexpr int GG_STAGES = 5;
-constexpr int GG_PATCHES = 2;                      // of an epilogue warp: 32 rows x 128 bytes each
 constexpr int GG_BK = 64;
 constexpr int GG_BOX_BYTES = GG_BK * 128;          // an MN-major box: 64 rows of K x 128 bytes
 constexpr int GG_A_BYTES = 128 * GG_BK * 2;        // 16 KB: this CTA's 128 of the tile's 256 rows (M)
-constexpr int GG_B_BYTES = 128 * GG_BK * 2;        // 16 KB: its 128 of the tile's 256 columns
-constexpr int GG_STAGE_BYTES = GG_A_BYTES + GG_B_BYTES;
 constexpr int GG_PATCH_BYTES = 32 * 128;
+constexpr int GG_MAX_STAGES = 5;
+// What depends on the tile: 256 columns (two accumulators), or WIDE, 512 (one accumulator of two halves)
+template <bool WIDE>
+struct GgTile {
+  static constexpr int NTILE = WIDE ? 512 : 256;
+  static constexpr int HALVES = NTILE / 256;                  // MMAs of 256 columns
+  static constexpr int STAGES = WIDE ? 4 : 5;
+  static constexpr int PATCHES = WIDE ? 1 : 2;                // of an epilogue warp: 32 rows x 128 bytes each
+  static constexpr int B_BYTES = HALVES * 128 * GG_BK * 2;    // this CTA's 128 of every 256 columns
+  static constexpr int STAGE_BYTES = GG_A_BYTES + B_BYTES;
+};
 constexpr int kGradChunk = 512;
 static_assert(kGradChunk % GG_BK == 0, "pieces are whole K steps");
 // registers move from the first warpgroup to the epilogue, whose fp32 sums take 128; the increase draws on what the block
@@ -51,16 +61,19 @@ static_assert(128 * GG_REG_LO + 32 * GG_EPI_WARPS * GG_REG_HI <= GG_THREADS * ((
               "setmaxnreg.inc would wait for registers that the CTA's pool never holds");
 
 struct GgShared {
-  uint64_t full[GG_STAGES];        // leader's: both CTAs' operands of the stage are there (one arrival from each)
-  uint64_t empty[GG_STAGES];       // the MMAs that read the stage are complete
-  uint64_t tail[GG_STAGES];        // this CTA's operands of a step that reaches past its group's end are there
+  uint64_t full[GG_MAX_STAGES];    // leader's: both CTAs' operands of the stage are there (one arrival from each)
+  uint64_t empty[GG_MAX_STAGES];   // the MMAs that read the stage are complete
+  uint64_t tail[GG_MAX_STAGES];    // this CTA's operands of a step that reaches past its group's end are there
   uint64_t tmem_full[2];
-  uint64_t tmem_empty[2];          // leader's: all epilogue warps of both CTAs have read the accumulator
+  uint64_t tmem_empty[2];          // leader's: all epilogue warps of both CTAs have read the accumulator (WIDE: the half of it)
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr size_t GG_SMEM_BYTES = 1024 + (size_t)GG_STAGES * GG_STAGE_BYTES + GG_PATCHES * GG_EPI_WARPS * GG_PATCH_BYTES + sizeof(GgShared);
-static_assert(GG_SMEM_BYTES <= 232448, "more than the 227 KB of shared memory a CTA can have");
+template <bool WIDE>
+constexpr size_t gg_smem_bytes() {
+  return 1024 + (size_t)GgTile<WIDE>::STAGES * GgTile<WIDE>::STAGE_BYTES + GgTile<WIDE>::PATCHES * GG_EPI_WARPS * GG_PATCH_BYTES + sizeof(GgShared);
+}
+static_assert(gg_smem_bytes<false>() <= 232448 && gg_smem_bytes<true>() <= 232448, "more than the 227 KB of shared memory a CTA can have");
 
 struct GgArgs {
   const int32_t* offsets;  // rows of group g: [offsets[g], offsets[g+1]); NULL = the `groups` even parts of [0, P)
@@ -142,12 +155,16 @@ __device__ __forceinline__ void gg_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// ROWS = false: weight gradient, true: row product.  F32: results in fp32, else bf16
-template <bool ROWS, bool F32>
+// ROWS = false: weight gradient, true: row product.  F32: results in fp32, else bf16.  WIDE: tiles of 256 x 512 (bf16 weight gradients)
+template <bool ROWS, bool F32, bool WIDE>
 __global__ void __launch_bounds__(GG_THREADS, 1)
 gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
                  const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmC0,
                  const __grid_constant__ CUtensorMap tmC1, const __grid_constant__ CUtensorMap tmC2, const GgArgs a) {
+  static_assert(!WIDE || (!ROWS && !F32), "one accumulator is for results that leave it in one pass");
+  using Tile = GgTile<WIDE>;
+  constexpr int GG_STAGES = Tile::STAGES, GG_STAGE_BYTES = Tile::STAGE_BYTES, GG_PATCHES = Tile::PATCHES, HALVES = Tile::HALVES;
+  constexpr bool MOVE_REGS = F32 || WIDE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* patches = smem + (size_t)GG_STAGES * GG_STAGE_BYTES;
@@ -223,7 +240,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   // K steps that one accumulator takes
   auto piece = [&](int steps) { return F32 && !ROWS ? kGradChunk / GG_BK : steps; };
 
-  if (F32 && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GG_REG_LO));
+  if (MOVE_REGS && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GG_REG_LO));
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (one thread)
     if (lane == 0) {
@@ -235,7 +252,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const Item w = fixed(nx);
         if (t + pairs < items) nx = item_of(t + pairs);  // its row range is on the way while this item loads
         const CUtensorMap* tmB = w.seg == 2 ? &tmB1 : &tmB0;
-        const int m0 = w.mt * 256 + rank * 128, n0 = w.nt * 256 + rank * 128;
+        const int m0 = w.mt * 256 + rank * 128, n0 = w.nt * Tile::NTILE + rank * 128;
         const bool tail = tail_rows(w) != 0;
         const int once = steps_once(w), steps = once * a.kparts;
         int r = w.beg, brow = w.beg, acol = ROWS ? 0 : w.seg * a.M + m0, left = once;
@@ -254,8 +271,9 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           } else {
             gg_load_pair(sa, &tmA, acol / 64, r, bar);
           }
-          if (a.b_pairs) {
-            gg_load_pair(sb, tmB, n0 / 64, brow, bar);
+          if (WIDE || a.b_pairs) {
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) gg_load_pair(sb + h * 2 * GG_BOX_BYTES, tmB, n0 / 64 + h * 4, brow, bar);
           } else {
             gg_load(sb, tmB, n0, brow, bar);
             gg_load(sb + GG_BOX_BYTES, tmB, n0 + 64, brow, bar);
@@ -284,8 +302,8 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       int r = w.beg;
       for (int i0 = 0; i0 < steps && ok; i0 += per, ++n) {
         const int i1 = min(i0 + per, steps);
-        const uint32_t buf = n & 1, d = tmem_base + buf * 256;
-        if (!gg_wait(smem_u32(&sh->tmem_empty[buf]), ((n >> 1) & 1) ^ 1, abort_flag)) {
+        const uint32_t buf = WIDE ? 0 : n & 1, d = tmem_base + buf * 256;
+        if (!WIDE && !gg_wait(smem_u32(&sh->tmem_empty[buf]), ((n >> 1) & 1) ^ 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -297,16 +315,23 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           // (zeros behind the group's end were written by threads, of the other CTA too: to see theirs takes more than what a
           // copy's arrival gives)
           if (tail && w.end - r < GG_BK) asm volatile("fence.acq_rel.cluster;" ::: "memory");
-          if (lane == 0) {
-            tc_fence_after();
-            const uint64_t adesc = adesc0 + (uint64_t)(s * (GG_STAGE_BYTES >> 4)), bdesc = bdesc0 + (uint64_t)(s * (GG_STAGE_BYTES >> 4));
-            const int rows = w.end - r;
+          const uint64_t adesc = adesc0 + (uint64_t)(s * (GG_STAGE_BYTES >> 4)), bdesc = bdesc0 + (uint64_t)(s * (GG_STAGE_BYTES >> 4));
+          const int rows = w.end - r;
 #pragma unroll
-            for (int k16 = 0; k16 < GG_BK / 16; ++k16)  // +16 rows of 128 B (MN-major) or +32 B inside the swizzle atom (K-major)
-              if (k16 * 16 < rows)
-                gg_mma(d, adesc + (uint64_t)(k16 * (ROWS ? 2 : 128)), bdesc + (uint64_t)(k16 * 128), idesc, (i > i0 || k16 > 0) ? 1u : 0u);
-            gg_commit(smem_u32(&sh->empty[0]) + s * 8);
+          for (int h = 0; h < HALVES; ++h) {
+            // (WIDE: the half is free once its last values are in the epilogue's registers)
+            if (WIDE && i == i0 && !gg_wait(smem_u32(&sh->tmem_empty[h]), (n & 1) ^ 1, abort_flag)) ok = false;
+            if (ok && lane == 0) {
+              tc_fence_after();
+#pragma unroll
+              for (int k16 = 0; k16 < GG_BK / 16; ++k16)  // +16 rows of 128 B (MN-major) or +32 B inside the swizzle atom (K-major)
+                if (k16 * 16 < rows)
+                  gg_mma(d + h * 256, adesc + (uint64_t)(k16 * (ROWS ? 2 : 128)), bdesc + (uint64_t)(h * (2 * GG_BOX_BYTES >> 4) + k16 * 128), idesc,
+                         (i > i0 || k16 > 0) ? 1u : 0u);
+            }
           }
+          if (!ok) break;
+          if (lane == 0) gg_commit(smem_u32(&sh->empty[0]) + s * 8);
           r += GG_BK;
           if (r >= w.end) r = w.beg;
           if (++s == GG_STAGES) s = 0, ph ^= 1;
@@ -334,7 +359,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const int end = ((rows + 15) & ~15) * 8;  // in 16-byte units of a box
       for (int i = rows * 8 + lane; i < end; i += 32) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) box[b * (GG_BOX_BYTES / 16) + i] = make_uint4(0, 0, 0, 0);
+        for (int b = 0; b < GG_STAGE_BYTES / GG_BOX_BYTES; ++b) box[b * (GG_BOX_BYTES / 16) + i] = make_uint4(0, 0, 0, 0);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -342,7 +367,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue
-    if (F32) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(GG_REG_HI));
+    if (MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(GG_REG_HI));
     const int q = warp & 3, cg = (warp - 4) >> 2;
     uint8_t* const patch0 = patches + (warp - 4) * (GG_PATCHES * GG_PATCH_BYTES);
     const uint32_t tmem_empty_leader = gg_in_cta(smem_u32(&sh->tmem_empty[0]), 0);
@@ -367,9 +392,9 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const Item w = fixed(nx);
       if (t + pairs < items) nx = item_of(t + pairs);
       const CUtensorMap* map = w.seg == 0 ? &tmC0 : w.seg == 1 ? &tmC1 : &tmC2;
-      const int mrow = w.mt * 256 + rank * 128 + q * 32, row = w.g * a.out_rows + mrow, col0 = w.nt * 256 + cg * 128;
+      const int mrow = w.mt * 256 + rank * 128 + q * 32, row = w.g * a.out_rows + mrow, col0 = w.nt * Tile::NTILE + cg * 128;
       const bool rows_here = mrow < a.M;
-      const int cols = rows_here ? min(128, a.N - col0) : 0;  // columns of this warp that exist
+      const int cols = rows_here ? min(128, a.N - col0) : 0;  // columns of this warp that exist (in the first 256)
       if (w.beg >= w.end) {
         // An expert without rows: zeros, not tile by tile but in runs (the 16 warps of the pair share the item's part of the
         // expert's matrix, 16-byte units [u, end) each), straight from patches that are cleared once.
@@ -450,8 +475,8 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           }
         }
       } else {
-        const uint32_t buf = n & 1;
-        if (!gg_wait(smem_u32(&sh->tmem_full[buf]), (n >> 1) & 1, abort_flag)) {
+        const uint32_t buf = WIDE ? 0 : n & 1;
+        if (!gg_wait(smem_u32(&sh->tmem_full[buf]), (WIDE ? n : n >> 1) & 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -462,39 +487,46 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(x), __uint_as_float(y));
           return *reinterpret_cast<const uint32_t*>(&b);
         };
-        // all 128 columns leave tensor memory before the first store, so that the accumulator goes back early
-        uint32_t o[64];
+        // all columns leave tensor memory before the first store, so that the accumulator goes back early
+        uint32_t o[HALVES][64];
 #pragma unroll
-        for (int c = 0; c < 128; c += 64) {
-          uint32_t v0[16], v1[16], v2[16], v3[16];
-          tc_ld_issue(tb + c, v0);
-          tc_ld_issue(tb + c + 16, v1);
-          tc_ld_issue(tb + c + 32, v2);
-          tc_ld_issue(tb + c + 48, v3);
-          tc_ld_wait(v0, v1);
-          tc_ld_wait(v2, v3);
+        for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            o[c / 2 + i] = pack(v0[2 * i], v0[2 * i + 1]);
-            o[c / 2 + 8 + i] = pack(v1[2 * i], v1[2 * i + 1]);
-            o[c / 2 + 16 + i] = pack(v2[2 * i], v2[2 * i + 1]);
-            o[c / 2 + 24 + i] = pack(v3[2 * i], v3[2 * i + 1]);
-          }
-        }
-        release(buf);
-        if (cols > 0) {
-          uint4* p = take_patches();
-#pragma unroll
-          for (int h = 0; h < GG_PATCHES; ++h)
+          for (int c = 0; c < 128; c += 64) {
+            uint32_t v0[16], v1[16], v2[16], v3[16];
+            tc_ld_issue(tb + h * 256 + c, v0);
+            tc_ld_issue(tb + h * 256 + c + 16, v1);
+            tc_ld_issue(tb + h * 256 + c + 32, v2);
+            tc_ld_issue(tb + h * 256 + c + 48, v3);
+            tc_ld_wait(v0, v1);
+            tc_ld_wait(v2, v3);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const int c = (h * PER) / 2 + 4 * i;
-              put(p + h * (GG_PATCH_BYTES / 16), i, make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]));
+              o[h][c / 2 + i] = pack(v0[2 * i], v0[2 * i + 1]);
+              o[h][c / 2 + 8 + i] = pack(v1[2 * i], v1[2 * i + 1]);
+              o[h][c / 2 + 16 + i] = pack(v2[2 * i], v2[2 * i + 1]);
+              o[h][c / 2 + 24 + i] = pack(v3[2 * i], v3[2 * i + 1]);
+            }
+          }
+          release(WIDE ? h : buf);
+        }
+#pragma unroll
+        for (int c0 = 0; c0 < HALVES * 128; c0 += GG_PATCHES * PER) {
+          const int h = c0 / 128, col = col0 + h * 256 + c0 % 128;
+          if (!rows_here || col >= a.N) break;  // uniform over the warp
+          uint4* p = take_patches();
+#pragma unroll
+          for (int t2 = 0; t2 < GG_PATCHES; ++t2)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int c = (c0 % 128 + t2 * PER) / 2 + 4 * i;
+              put(p + t2 * (GG_PATCH_BYTES / 16), i, make_uint4(o[h][c], o[h][c + 1], o[h][c + 2], o[h][c + 3]));
             }
           patches_written();
           if (lane == 0) {
-            gg_store(map, col0, row, smem_u32(p), a.add);
-            if (PER < cols) gg_store(map, col0 + PER, row, smem_u32(p) + GG_PATCH_BYTES, a.add);
+#pragma unroll
+            for (int t2 = 0; t2 < GG_PATCHES; ++t2)
+              if (col + t2 * PER < a.N) gg_store(map, col + t2 * PER, row, smem_u32(p) + t2 * GG_PATCH_BYTES, a.add);
             sent();
           }
         }
@@ -549,19 +581,19 @@ bool gg_make_b_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t col
   return cols % 64 == 0 ? gg_make_chunk_map(m, base, rows, cols) : gg_make_map(m, base, false, rows, cols, GG_BK);
 }
 
-template <bool ROWS, bool F32>
+template <bool ROWS, bool F32, bool WIDE = false>
 int gg_launch(const CUtensorMap (&tm)[6], const GgArgs& a, cudaStream_t st) {
   static bool attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200MOE_EDRIVER;
   if (!attr_set[dev]) {  // per-device attribute
-    cudaFuncSetAttribute(gemm_grad_kernel<ROWS, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GG_SMEM_BYTES);
+    cudaFuncSetAttribute(gemm_grad_kernel<ROWS, F32, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gg_smem_bytes<WIDE>());
     attr_set[dev] = true;
   }
   const int64_t items = (int64_t)a.groups * a.segs * a.MT * a.NT;
   if (items >= (int64_t(1) << 31)) return B200MOE_ESHAPE;
   const int pairs = std::max(1, moe_device_sm_count() / 2);
-  return moe_launch_clusters(true, dim3(2, 1, 1), gemm_grad_kernel<ROWS, F32>, (unsigned)(2 * (items < pairs ? items : pairs)), GG_THREADS, GG_SMEM_BYTES, st, tm[0],
+  return moe_launch_clusters(true, dim3(2, 1, 1), gemm_grad_kernel<ROWS, F32, WIDE>, (unsigned)(2 * (items < pairs ? items : pairs)), GG_THREADS, gg_smem_bytes<WIDE>(), st, tm[0],
                        tm[1], tm[2], tm[3], tm[4], tm[5], a);
 }
 
@@ -582,13 +614,15 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   a.P = (int)g.P;
   a.groups = g.groups, a.segs = g.segs;
   a.M = g.M, a.N = g.N;
-  a.MT = (g.M + 255) / 256, a.NT = (g.N + 255) / 256;
+  const bool wide = !g.out_f32 && g.N % 64 == 0 && GGWIDE;
+  a.MT = (g.M + 255) / 256, a.NT = (g.N + (wide ? 511 : 255)) / (wide ? 512 : 256);
   a.out_rows = g.M;
   a.kparts = g.kparts, a.kpart_cols = g.M;
   a.out0 = reinterpret_cast<uint8_t*>(g.out[0]), a.out1 = reinterpret_cast<uint8_t*>(g.out[1]), a.out2 = reinterpret_cast<uint8_t*>(g.out[2]);
   a.add = g.add;
   a.b_pairs = g.N % 64 == 0;
   a.status = g.status;
+  if (wide) return gg_launch<false, false, true>(tm, a, st);
   return g.out_f32 ? gg_launch<false, true>(tm, a, st) : gg_launch<false, false>(tm, a, st);
 }
 
