@@ -211,6 +211,16 @@ def test_linear_w8_backward(ops, M, K, N, scale_dtype):
     assert int(st.item()) == 0
 
 
+def test_linear_w8_backward_of_many_rows(ops):
+    """bf16 weight gradients of more rows than one accumulator takes."""
+    g = gen(12)
+    M, K, N = 40000, 256, 192
+    dy, x = randn(g, M, N).abs(), randn(g, M, K).abs()        # terms of one sign: the sum's error does not average out
+    low = ops.linear_w8_backward(dy, x, dw=torch.empty(N, K, dtype=torch.bfloat16, device=DEV))[1]
+    want = dy.double().t() @ x.double()
+    within(low, want, rounded(want, G.product_bound(dy.double().t(), x.double(), 512 + M // 512), torch.bfloat16), "dw bf16")
+
+
 def test_linear_w8_backward_of_small_gradients(ops):
     """Rows that are tiny throughout keep their bits: the scale's floor is for gradients."""
     g = gen(11)

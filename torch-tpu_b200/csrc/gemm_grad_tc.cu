@@ -23,15 +23,12 @@
 // The tensor cores' fp32 accumulation is not an IEEE one: against fp64 the error of a sum of K products grows with K (measured,
 // random operands: 1e-6 of the result's norm at K = 1024, 4.4e-6 at 4096, 1.9e-5 at 16384).  fp32 results are therefore formed
 // in pieces of kGradChunk rows that the epilogue adds up, in order, in IEEE fp32 registers.  bf16 results round more than
-// that away and take all rows in one piece.
+// that away and take all rows in one piece, up to kGradOnePiece of them.
 //
 // Every wait is bounded; on a time-out status bit 1 is raised and all roles leave.
 #include <algorithm>
 
 #include "tc_ptx.cuh"
-#ifndef GGWIDE
-#define GGWIDE 1
-#endif
 
 namespace {
 
@@ -53,6 +50,7 @@ struct GgTile {
   static constexpr int STAGE_BYTES = GG_A_BYTES + B_BYTES;
 };
 constexpr int kGradChunk = 512;
+constexpr int64_t kGradOnePiece = 32768;  // (4e-5 of the result's norm, 2e-4 where all terms have one sign; bf16 rounds at 2e-3)
 static_assert(kGradChunk % GG_BK == 0, "pieces are whole K steps");
 // registers move from the first warpgroup to the epilogue, whose fp32 sums take 128; the increase draws on what the block
 // was launched with
@@ -155,16 +153,18 @@ __device__ __forceinline__ void gg_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// ROWS = false: weight gradient, true: row product.  F32: results in fp32, else bf16.  WIDE: tiles of 256 x 512 (bf16 weight gradients)
-template <bool ROWS, bool F32, bool WIDE>
+// ROWS = false: weight gradient, true: row product.  PIECES: sums in pieces of kGradChunk rows.  F32: results in fp32, else bf16.  WIDE:
+// tiles of 256 x 512
+template <bool ROWS, bool PIECES, bool F32, bool WIDE>
 __global__ void __launch_bounds__(GG_THREADS, 1)
 gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
                  const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmC0,
                  const __grid_constant__ CUtensorMap tmC1, const __grid_constant__ CUtensorMap tmC2, const GgArgs a) {
-  static_assert(!WIDE || (!ROWS && !F32), "one accumulator is for results that leave it in one pass");
+  static_assert(!WIDE || !PIECES, "one accumulator is for results that leave it in one pass");
+  static_assert(!F32 || PIECES, "");
   using Tile = GgTile<WIDE>;
   constexpr int GG_STAGES = Tile::STAGES, GG_STAGE_BYTES = Tile::STAGE_BYTES, GG_PATCHES = Tile::PATCHES, HALVES = Tile::HALVES;
-  constexpr bool MOVE_REGS = F32 || WIDE;
+  constexpr bool MOVE_REGS = PIECES || WIDE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* patches = smem + (size_t)GG_STAGES * GG_STAGE_BYTES;
@@ -238,7 +238,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   };
   auto steps_once = [&](const Item& w) { return (max(w.end - w.beg, 0) + GG_BK - 1) / GG_BK; };
   // K steps that one accumulator takes
-  auto piece = [&](int steps) { return F32 && !ROWS ? kGradChunk / GG_BK : steps; };
+  auto piece = [&](int steps) { return PIECES ? kGradChunk / GG_BK : steps; };
 
   if (MOVE_REGS && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GG_REG_LO));
   if (warp == 0) {
@@ -428,7 +428,11 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         __syncwarp();
         if (lane == 0) gg_arrive_read(tmem_empty_leader + buf * 8);
       };
-      if constexpr (F32) {
+      auto pack = [](uint32_t x, uint32_t y) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(x), __uint_as_float(y));
+        return *reinterpret_cast<const uint32_t*>(&b);
+      };
+      if constexpr (PIECES) {
         float acc[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) acc[i] = 0.f;
@@ -463,9 +467,11 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           for (int h = 0; h < GG_PATCHES; ++h)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const int c = c0 + h * PER + 4 * i;
-              put(p + h * (GG_PATCH_BYTES / 16), i, make_uint4(__float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]),
-                                                               __float_as_uint(acc[c + 3])));
+              const int c = c0 + h * PER + (F32 ? 4 : 8) * i;
+              auto at = [&](int k) { return __float_as_uint(acc[c + k]); };
+              put(p + h * (GG_PATCH_BYTES / 16), i, F32 ? make_uint4(at(0), at(1), at(2), at(3))
+                                                        : make_uint4(pack(at(0), at(1)), pack(at(F32 ? 0 : 2), at(F32 ? 0 : 3)),
+                                                                     pack(at(F32 ? 0 : 4), at(F32 ? 0 : 5)), pack(at(F32 ? 0 : 6), at(F32 ? 0 : 7))));
             }
           patches_written();
           if (lane == 0) {
@@ -483,10 +489,6 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         ++n;
         tc_fence_after();
         const uint32_t tb = tmem_base + ((uint32_t)(q * 32) << 16) + buf * 256 + cg * 128;
-        auto pack = [](uint32_t x, uint32_t y) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(x), __uint_as_float(y));
-          return *reinterpret_cast<const uint32_t*>(&b);
-        };
         // all columns leave tensor memory before the first store, so that the accumulator goes back early
         uint32_t o[HALVES][64];
 #pragma unroll
@@ -581,19 +583,19 @@ bool gg_make_b_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t col
   return cols % 64 == 0 ? gg_make_chunk_map(m, base, rows, cols) : gg_make_map(m, base, false, rows, cols, GG_BK);
 }
 
-template <bool ROWS, bool F32, bool WIDE = false>
+template <bool ROWS, bool PIECES, bool F32, bool WIDE>
 int gg_launch(const CUtensorMap (&tm)[6], const GgArgs& a, cudaStream_t st) {
   static bool attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200MOE_EDRIVER;
   if (!attr_set[dev]) {  // per-device attribute
-    cudaFuncSetAttribute(gemm_grad_kernel<ROWS, F32, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gg_smem_bytes<WIDE>());
+    cudaFuncSetAttribute(gemm_grad_kernel<ROWS, PIECES, F32, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gg_smem_bytes<WIDE>());
     attr_set[dev] = true;
   }
   const int64_t items = (int64_t)a.groups * a.segs * a.MT * a.NT;
   if (items >= (int64_t(1) << 31)) return B200MOE_ESHAPE;
   const int pairs = std::max(1, moe_device_sm_count() / 2);
-  return moe_launch_clusters(true, dim3(2, 1, 1), gemm_grad_kernel<ROWS, F32, WIDE>, (unsigned)(2 * (items < pairs ? items : pairs)), GG_THREADS, gg_smem_bytes<WIDE>(), st, tm[0],
+  return moe_launch_clusters(true, dim3(2, 1, 1), gemm_grad_kernel<ROWS, PIECES, F32, WIDE>, (unsigned)(2 * (items < pairs ? items : pairs)), GG_THREADS, gg_smem_bytes<WIDE>(), st, tm[0],
                        tm[1], tm[2], tm[3], tm[4], tm[5], a);
 }
 
@@ -614,16 +616,25 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   a.P = (int)g.P;
   a.groups = g.groups, a.segs = g.segs;
   a.M = g.M, a.N = g.N;
-  const bool wide = !g.out_f32 && g.N % 64 == 0 && GGWIDE;
-  a.MT = (g.M + 255) / 256, a.NT = (g.N + (wide ? 511 : 255)) / (wide ? 512 : 256);
+  // bf16 results: tiles of 512 columns move three quarters of the operand bytes per product, so a wide tile takes 1 / 1.15 of the
+  // time of two narrow ones where their number fills the rounds of CTA pairs equally well.  Narrow / wide, us (rows x output):
+  // 1024 x 43008 x 4096 283 / 250, 4096 x 2048 x 4096 56.4 / 50.6, 2048 x 4096 x 7168 94.2 / 91.7; with worse filled rounds, or columns
+  // that are not there, 4096 x 1024 x 1024 28.4 / 45.2, 2048 x 2048 x 2048 21.0 / 27.6, 4096 x 14336 x 1280 113 / 130.
+  a.MT = (g.M + 255) / 256;
+  const int64_t pairs = std::max(1, moe_device_sm_count() / 2), row_tiles = (int64_t)g.groups * g.segs * a.MT;
+  auto rounds = [&](int width) { return (row_tiles * ((g.N + width - 1) / width) + pairs - 1) / pairs; };
+  const bool pieces = g.out_f32 || g.P > kGradOnePiece;
+  const bool wide = !pieces && g.N % 64 == 0 && rounds(512) * 2 * 100 <= rounds(256) * 115;
+  a.NT = (g.N + (wide ? 511 : 255)) / (wide ? 512 : 256);
   a.out_rows = g.M;
   a.kparts = g.kparts, a.kpart_cols = g.M;
   a.out0 = reinterpret_cast<uint8_t*>(g.out[0]), a.out1 = reinterpret_cast<uint8_t*>(g.out[1]), a.out2 = reinterpret_cast<uint8_t*>(g.out[2]);
   a.add = g.add;
   a.b_pairs = g.N % 64 == 0;
   a.status = g.status;
-  if (wide) return gg_launch<false, false, true>(tm, a, st);
-  return g.out_f32 ? gg_launch<false, true>(tm, a, st) : gg_launch<false, false>(tm, a, st);
+  if (g.out_f32) return gg_launch<false, true, true, false>(tm, a, st);
+  if (pieces) return gg_launch<false, true, false, false>(tm, a, st);
+  return wide ? gg_launch<false, false, false, true>(tm, a, st) : gg_launch<false, false, false, false>(tm, a, st);
 }
 
 int moe_row_product_tc(__nv_bfloat16* out, bool add, const __nv_bfloat16* a16, int lda, const __nv_bfloat16* b, int64_t rows, int K, int b_rows,
@@ -642,5 +653,5 @@ int moe_row_product_tc(__nv_bfloat16* out, bool add, const __nv_bfloat16* a16, i
   a.b_pairs = N % 64 == 0;
   a.K = K, a.kb_rows = b_cycle;
   a.status = status;
-  return gg_launch<true, false>(tm, a, st);
+  return gg_launch<true, false, false, false>(tm, a, st);
 }
