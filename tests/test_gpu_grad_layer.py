@@ -143,6 +143,29 @@ def test_layer_backward_replayed_from_a_graph():
     assert int(layer.status.item()) == 0
 
 
+def test_small_batch_replayed_from_a_graph():
+    """dx of few pairs: a K range that is split, its partial sums cleared and added inside the graph."""
+    layer, x, dout, _ = make_layer(T=12, H=512, I=1024, E=4, k=2)
+    sx, sd = x.clone(), dout.clone()
+    layer.backward(sx, sd)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = layer.backward(sx, sd)
+    for seed in (1, 2, 3):
+        h = gen(seed)
+        sx.copy_(randn(h, 12, 512)), sd.copy_(randn(h, 12, 512, scale=1e-2))
+        graph.replay()
+        torch.cuda.synchronize()
+        e = G.experts_backward(sd, sx, *layer.w, layer.ids[:12], layer.topk_w[:12])
+        dl, bl = G.route_backward(e["dw"][0], layer.logits[:12], layer.ids[:12], "softmax", True, 1.0, dw_bound=e["dw"][1])
+        within(res.dlogits, dl, bl, "dlogits")
+        rx, bx, _, _ = G.router_backward(dl, sx, layer.router_w)
+        half = G.half_step(torch.bfloat16)
+        bound = e["dx"][1] + (e["dx"][0].abs() + e["dx"][1]) * half + bx + bl @ layer.router_w.double().abs() + (rx.abs() + bx) * half
+        within(res.dx, e["dx"][0] + rx, rounded(e["dx"][0] + rx, bound, torch.bfloat16), "dx")
+
+
 def test_two_calls_at_once_on_two_streams():
     """Calls on different streams with workspaces of their own."""
     import torch_tpu_b200

@@ -39,15 +39,16 @@ constexpr int GG_BOX_BYTES = GG_BK * 128;          // an MN-major box: 64 rows o
 constexpr int GG_A_BYTES = 128 * GG_BK * 2;        // 16 KB: this CTA's 128 of the tile's 256 rows (M)
 constexpr int GG_PATCH_BYTES = 32 * 128;
 constexpr int GG_MAX_STAGES = 5;
-// What depends on the tile: 256 columns (two accumulators), or WIDE, 512 (one accumulator of two halves)
-template <bool WIDE>
+// What depends on the tile: 256 columns (two accumulators), or WIDE, 512 (one accumulator of two halves); NA: tiles of A that a K
+// step multiplies with its tile of B, one after the other into the same accumulator (columns kpart_cols apart)
+template <bool WIDE, int NA>
 struct GgTile {
   static constexpr int NTILE = WIDE ? 512 : 256;
   static constexpr int HALVES = NTILE / 256;                  // MMAs of 256 columns
-  static constexpr int STAGES = WIDE ? 4 : 5;
-  static constexpr int PATCHES = WIDE ? 1 : 2;                // of an epilogue warp: 32 rows x 128 bytes each
+  static constexpr int STAGES = NA == 3 ? 3 : WIDE ? 4 : 5;
+  static constexpr int PATCHES = WIDE || NA == 3 ? 1 : 2;                // of an epilogue warp: 32 rows x 128 bytes each
   static constexpr int B_BYTES = HALVES * 128 * GG_BK * 2;    // this CTA's 128 of every 256 columns
-  static constexpr int STAGE_BYTES = GG_A_BYTES + B_BYTES;
+  static constexpr int STAGE_BYTES = NA * GG_A_BYTES + B_BYTES;
 };
 constexpr int kGradChunk = 512;
 constexpr int64_t kGradOnePiece = 32768;  // (4e-5 of the result's norm, 2e-4 where all terms have one sign; bf16 rounds at 2e-3)
@@ -67,18 +68,19 @@ struct GgShared {
   uint32_t tmem_base;
   int abort_flag;
 };
-template <bool WIDE>
+template <bool WIDE, int NA>
 constexpr size_t gg_smem_bytes() {
-  return 1024 + (size_t)GgTile<WIDE>::STAGES * GgTile<WIDE>::STAGE_BYTES + GgTile<WIDE>::PATCHES * GG_EPI_WARPS * GG_PATCH_BYTES + sizeof(GgShared);
+  using Tile = GgTile<WIDE, NA>;
+  return 1024 + (size_t)Tile::STAGES * Tile::STAGE_BYTES + Tile::PATCHES * GG_EPI_WARPS * GG_PATCH_BYTES + sizeof(GgShared);
 }
-static_assert(gg_smem_bytes<false>() <= 232448 && gg_smem_bytes<true>() <= 232448, "more than the 227 KB of shared memory a CTA can have");
+static_assert(gg_smem_bytes<false, 1>() <= 232448 && gg_smem_bytes<true, 1>() <= 232448 && gg_smem_bytes<false, 3>() <= 232448, "more than the 227 KB of shared memory a CTA can have");
 
 struct GgArgs {
   const int32_t* offsets;  // rows of group g: [offsets[g], offsets[g+1]); NULL = the `groups` even parts of [0, P)
   int P, groups, segs;     // segs: operand pairs that a group has (columns [seg * M, (seg + 1) * M) of A)
   int M, N, MT, NT;        // outputs of one (group, segment); tiles along both
   int out_rows;            // rows of the output between groups
-  int kparts, kpart_cols;  // the K range is walked kparts times, with columns of A kpart_cols further each time
+  int kpart_cols;          // NA > 1: columns between A's ranges
   int K;                   // row product: depth; B's row of step k is k % kb_rows
   int kb_rows;
   int b_pairs;             // B's maps are of 64-column chunks (whole ones: N % 64 == 0)
@@ -154,15 +156,16 @@ __device__ __forceinline__ void gg_cluster_sync() {
 }
 
 // ROWS = false: weight gradient, true: row product.  PIECES: sums in pieces of kGradChunk rows.  F32: results in fp32, else bf16.  WIDE:
-// tiles of 256 x 512
-template <bool ROWS, bool PIECES, bool F32, bool WIDE>
+// tiles of 256 x 512.  NA = 3: the sum is over three column ranges of A as well (the router's dlogits)
+template <bool ROWS, bool PIECES, bool F32, bool WIDE, int NA>
 __global__ void __launch_bounds__(GG_THREADS, 1)
 gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
                  const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmC0,
                  const __grid_constant__ CUtensorMap tmC1, const __grid_constant__ CUtensorMap tmC2, const GgArgs a) {
   static_assert(!WIDE || !PIECES, "one accumulator is for results that leave it in one pass");
   static_assert(!F32 || PIECES, "");
-  using Tile = GgTile<WIDE>;
+  static_assert(NA == 1 || (!ROWS && !WIDE), "");
+  using Tile = GgTile<WIDE, NA>;
   constexpr int GG_STAGES = Tile::STAGES, GG_STAGE_BYTES = Tile::STAGE_BYTES, GG_PATCHES = Tile::PATCHES, HALVES = Tile::HALVES;
   constexpr bool MOVE_REGS = PIECES || WIDE;
   extern __shared__ uint8_t smem_raw[];
@@ -234,9 +237,9 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   // rows of the item's last K step, if some of the rows that its MMAs read there are not the group's (0: none are)
   auto tail_rows = [&](const Item& w) {
     const int last = (w.end - w.beg) & (GG_BK - 1);
-    return !ROWS && a.kparts == 1 && w.end < a.P && (last & 15) ? last : 0;
+    return !ROWS && NA == 1 && w.end < a.P && (last & 15) ? last : 0;
   };
-  auto steps_once = [&](const Item& w) { return (max(w.end - w.beg, 0) + GG_BK - 1) / GG_BK; };
+  auto steps_of = [&](const Item& w) { return (max(w.end - w.beg, 0) + GG_BK - 1) / GG_BK; };
   // K steps that one accumulator takes
   auto piece = [&](int steps) { return PIECES ? kGradChunk / GG_BK : steps; };
 
@@ -254,14 +257,14 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const CUtensorMap* tmB = w.seg == 2 ? &tmB1 : &tmB0;
         const int m0 = w.mt * 256 + rank * 128, n0 = w.nt * Tile::NTILE + rank * 128;
         const bool tail = tail_rows(w) != 0;
-        const int once = steps_once(w), steps = once * a.kparts;
-        int r = w.beg, brow = w.beg, acol = ROWS ? 0 : w.seg * a.M + m0, left = once;
+        const int steps = steps_of(w), acol = ROWS ? 0 : w.seg * a.M + m0;
+        int r = w.beg, brow = w.beg;
         for (int i = 0; i < steps; ++i) {
           if (!mbar_wait(smem_u32(&sh->empty[0]) + s * 8, ph, abort_flag)) {
             ok = false;
             break;
           }
-          const uint32_t sa = smem_base + s * GG_STAGE_BYTES, sb = sa + GG_A_BYTES;
+          const uint32_t sa = smem_base + s * GG_STAGE_BYTES, sb = sa + NA * GG_A_BYTES;
           // to the leader's barrier, or (the step whose tail has to be cleared first) to this CTA's own
           const uint32_t bar = tail && w.end - r < GG_BK ? gg_in_cta(smem_u32(&sh->tail[0]) + s * 8, rank)
                                                          : gg_in_cta(smem_u32(&sh->full[0]) + s * 8, 0);
@@ -269,7 +272,8 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (ROWS) {
             gg_load(sa, &tmA, r, m0, bar);
           } else {
-            gg_load_pair(sa, &tmA, acol / 64, r, bar);
+#pragma unroll
+            for (int k = 0; k < NA; ++k) gg_load_pair(sa + k * GG_A_BYTES, &tmA, (acol + k * a.kpart_cols) / 64, r, bar);
           }
           if (WIDE || a.b_pairs) {
 #pragma unroll
@@ -280,7 +284,6 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           }
           r += GG_BK, brow += GG_BK;
           if (ROWS && brow == a.kb_rows) brow = 0;
-          if (!ROWS && --left == 0) left = once, r = brow = w.beg, acol += a.kpart_cols;
           if (++s == GG_STAGES) s = 0, ph ^= 1;
         }
       }
@@ -289,7 +292,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     // ------------------------------------------------------------------ MMA issuer (one thread; the warp stays together)
     const uint32_t idesc = gg_idesc(ROWS ? 0 : 1);
     const uint64_t adesc0 = ROWS ? make_smem_desc(smem_base, 16, 1024) : make_smem_desc(smem_base, GG_BOX_BYTES, 1024);
-    const uint64_t bdesc0 = make_smem_desc(smem_base + GG_A_BYTES, GG_BOX_BYTES, 1024);
+    const uint64_t bdesc0 = make_smem_desc(smem_base + NA * GG_A_BYTES, GG_BOX_BYTES, 1024);
     uint32_t s = 0, ph = 0, n = 0;
     bool ok = true;
     Item nx{};
@@ -298,7 +301,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const Item w = fixed(nx);
       if (t + pairs < items) nx = item_of(t + pairs);
       const bool tail = tail_rows(w) != 0;
-      const int once = steps_once(w), steps = once * a.kparts, per = piece(steps);
+      const int steps = steps_of(w), per = piece(steps);
       int r = w.beg;
       for (int i0 = 0; i0 < steps && ok; i0 += per, ++n) {
         const int i1 = min(i0 + per, steps);
@@ -324,16 +327,17 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (ok && lane == 0) {
               tc_fence_after();
 #pragma unroll
-              for (int k16 = 0; k16 < GG_BK / 16; ++k16)  // +16 rows of 128 B (MN-major) or +32 B inside the swizzle atom (K-major)
-                if (k16 * 16 < rows)
-                  gg_mma(d + h * 256, adesc + (uint64_t)(k16 * (ROWS ? 2 : 128)), bdesc + (uint64_t)(h * (2 * GG_BOX_BYTES >> 4) + k16 * 128), idesc,
-                         (i > i0 || k16 > 0) ? 1u : 0u);
+              for (int k = 0; k < NA; ++k)
+#pragma unroll
+                for (int k16 = 0; k16 < GG_BK / 16; ++k16)  // +16 rows of 128 B (MN-major) or +32 B inside the swizzle atom (K-major)
+                  if (k16 * 16 < rows)
+                    gg_mma(d + h * 256, adesc + (uint64_t)(k * (GG_A_BYTES >> 4) + k16 * (ROWS ? 2 : 128)),
+                           bdesc + (uint64_t)(h * (2 * GG_BOX_BYTES >> 4) + k16 * 128), idesc, (i > i0 || k > 0 || k16 > 0) ? 1u : 0u);
             }
           }
           if (!ok) break;
           if (lane == 0) gg_commit(smem_u32(&sh->empty[0]) + s * 8);
           r += GG_BK;
-          if (r >= w.end) r = w.beg;
           if (++s == GG_STAGES) s = 0, ph ^= 1;
         }
         if (ok && lane == 0) gg_commit(smem_u32(&sh->tmem_full[buf]));
@@ -349,7 +353,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     for (int t = pair0; t < items; t += pairs) {
       const Item w = fixed(nx);
       if (t + pairs < items) nx = item_of(t + pairs);
-      at += (uint32_t)(steps_once(w) * a.kparts);
+      at += (uint32_t)steps_of(w);
       const int rows = w.beg < w.end ? tail_rows(w) : 0;
       if (!rows) continue;
       const uint32_t s = (at - 1) % GG_STAGES;
@@ -422,7 +426,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         continue;
       }
       auto put = [&](uint4* p, int i, uint4 v) { p[lane * 8 + (i ^ (lane & 7))] = v; };  // the 128-byte swizzle
-      const int steps = steps_once(w) * a.kparts, per = piece(steps);
+      const int steps = steps_of(w), per = piece(steps);
       auto release = [&](uint32_t buf) {  // the accumulator is in registers (or nobody wants it)
         tc_fence_before();
         __syncwarp();
@@ -475,8 +479,9 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           patches_written();
           if (lane == 0) {
-            gg_store(map, col0 + c0, row, smem_u32(p), a.add);
-            if (c0 + PER < cols) gg_store(map, col0 + c0 + PER, row, smem_u32(p) + GG_PATCH_BYTES, a.add);
+#pragma unroll
+            for (int h = 0; h < GG_PATCHES; ++h)
+              if (c0 + h * PER < cols) gg_store(map, col0 + c0 + h * PER, row, smem_u32(p) + h * GG_PATCH_BYTES, a.add);
             sent();
           }
         }
@@ -583,20 +588,30 @@ bool gg_make_b_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t col
   return cols % 64 == 0 ? gg_make_chunk_map(m, base, rows, cols) : gg_make_map(m, base, false, rows, cols, GG_BK);
 }
 
-template <bool ROWS, bool PIECES, bool F32, bool WIDE>
+template <bool ROWS, bool PIECES, bool F32, bool WIDE, int NA = 1>
 int gg_launch(const CUtensorMap (&tm)[6], const GgArgs& a, cudaStream_t st) {
   static bool attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200MOE_EDRIVER;
   if (!attr_set[dev]) {  // per-device attribute
-    cudaFuncSetAttribute(gemm_grad_kernel<ROWS, PIECES, F32, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gg_smem_bytes<WIDE>());
+    cudaFuncSetAttribute(gemm_grad_kernel<ROWS, PIECES, F32, WIDE, NA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gg_smem_bytes<WIDE, NA>());
     attr_set[dev] = true;
   }
   const int64_t items = (int64_t)a.groups * a.segs * a.MT * a.NT;
   if (items >= (int64_t(1) << 31)) return B200MOE_ESHAPE;
   const int pairs = std::max(1, moe_device_sm_count() / 2);
-  return moe_launch_clusters(true, dim3(2, 1, 1), gemm_grad_kernel<ROWS, PIECES, F32, WIDE>, (unsigned)(2 * (items < pairs ? items : pairs)), GG_THREADS, gg_smem_bytes<WIDE>(), st, tm[0],
+  return moe_launch_clusters(true, dim3(2, 1, 1), gemm_grad_kernel<ROWS, PIECES, F32, WIDE, NA>, (unsigned)(2 * (items < pairs ? items : pairs)), GG_THREADS, gg_smem_bytes<WIDE, NA>(), st, tm[0],
                        tm[1], tm[2], tm[3], tm[4], tm[5], a);
+}
+
+// Tiles of 512 columns move three quarters of the operand bytes per product, so a wide tile takes 1 / 1.15 of the time of two
+// narrow ones where their number fills the rounds of CTA pairs equally well.  bf16 weight gradients, narrow / wide, us (rows x
+// output): 1024 x 43008 x 4096 283 / 250, 4096 x 2048 x 4096 56.4 / 50.6, 2048 x 4096 x 7168 94.2 / 91.7; with worse filled rounds, or
+// columns that are not there, 4096 x 1024 x 1024 28.4 / 45.2, 2048 x 2048 x 2048 21.0 / 27.6, 4096 x 14336 x 1280 113 / 130.
+bool gg_wide(int64_t row_tiles, int N) {
+  const int64_t pairs = std::max(1, moe_device_sm_count() / 2);
+  auto rounds = [&](int width) { return (row_tiles * ((N + width - 1) / width) + pairs - 1) / pairs; };
+  return N % 64 == 0 && rounds(512) * 2 * 100 <= rounds(256) * 115;
 }
 
 }  // namespace
@@ -604,7 +619,8 @@ int gg_launch(const CUtensorMap (&tm)[6], const GgArgs& a, cudaStream_t st) {
 int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   CUtensorMap tm[6];
   if (g.M % 64) return B200MOE_ESHAPE;
-  if (g.kparts > 1 && (g.segs > 1 || g.offsets)) return B200MOE_EINVAL;  // (their ends are ends of the tensor or of whole steps)
+  // (three ranges: no tails, their ends are ends of the tensor or of whole steps)
+  if (g.kparts != 1 && !(g.kparts == 3 && g.segs == 1 && !g.offsets && g.out_f32)) return B200MOE_EINVAL;
   const int64_t acols = (int64_t)g.segs * g.M * g.kparts;
   if (!gg_make_chunk_map(&tm[0], g.a, (uint64_t)g.P, (uint64_t)acols)) return B200MOE_EDRIVER;
   if (!gg_make_b_map(&tm[1], g.b0, (uint64_t)g.P, (uint64_t)g.N)) return B200MOE_EDRIVER;
@@ -616,22 +632,17 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   a.P = (int)g.P;
   a.groups = g.groups, a.segs = g.segs;
   a.M = g.M, a.N = g.N;
-  // bf16 results: tiles of 512 columns move three quarters of the operand bytes per product, so a wide tile takes 1 / 1.15 of the
-  // time of two narrow ones where their number fills the rounds of CTA pairs equally well.  Narrow / wide, us (rows x output):
-  // 1024 x 43008 x 4096 283 / 250, 4096 x 2048 x 4096 56.4 / 50.6, 2048 x 4096 x 7168 94.2 / 91.7; with worse filled rounds, or columns
-  // that are not there, 4096 x 1024 x 1024 28.4 / 45.2, 2048 x 2048 x 2048 21.0 / 27.6, 4096 x 14336 x 1280 113 / 130.
-  a.MT = (g.M + 255) / 256;
-  const int64_t pairs = std::max(1, moe_device_sm_count() / 2), row_tiles = (int64_t)g.groups * g.segs * a.MT;
-  auto rounds = [&](int width) { return (row_tiles * ((g.N + width - 1) / width) + pairs - 1) / pairs; };
   const bool pieces = g.out_f32 || g.P > kGradOnePiece;
-  const bool wide = !pieces && g.N % 64 == 0 && rounds(512) * 2 * 100 <= rounds(256) * 115;
+  a.MT = (g.M + 255) / 256;
+  const bool wide = !pieces && gg_wide((int64_t)g.groups * g.segs * a.MT, g.N);
   a.NT = (g.N + (wide ? 511 : 255)) / (wide ? 512 : 256);
   a.out_rows = g.M;
-  a.kparts = g.kparts, a.kpart_cols = g.M;
+  a.kpart_cols = g.M;
   a.out0 = reinterpret_cast<uint8_t*>(g.out[0]), a.out1 = reinterpret_cast<uint8_t*>(g.out[1]), a.out2 = reinterpret_cast<uint8_t*>(g.out[2]);
   a.add = g.add;
   a.b_pairs = g.N % 64 == 0;
   a.status = g.status;
+  if (g.kparts == 3) return gg_launch<false, true, true, false, 3>(tm, a, st);
   if (g.out_f32) return gg_launch<false, true, true, false>(tm, a, st);
   if (pieces) return gg_launch<false, true, false, false>(tm, a, st);
   return wide ? gg_launch<false, false, false, true>(tm, a, st) : gg_launch<false, false, false, false>(tm, a, st);
@@ -647,11 +658,12 @@ int moe_row_product_tc(__nv_bfloat16* out, bool add, const __nv_bfloat16* a16, i
   GgArgs a{};
   a.groups = a.segs = 1;
   a.M = (int)rows, a.N = N;
-  a.MT = (int)((rows + 255) / 256), a.NT = (N + 255) / 256;
-  a.kparts = 1;
+  a.MT = (int)((rows + 255) / 256);
+  const bool wide = gg_wide(a.MT, N);
+  a.NT = (N + (wide ? 511 : 255)) / (wide ? 512 : 256);
   a.add = add;
   a.b_pairs = N % 64 == 0;
   a.K = K, a.kb_rows = b_cycle;
   a.status = status;
-  return gg_launch<true, false, false, false>(tm, a, st);
+  return wide ? gg_launch<true, false, false, true>(tm, a, st) : gg_launch<true, false, false, false>(tm, a, st);
 }
