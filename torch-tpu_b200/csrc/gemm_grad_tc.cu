@@ -22,7 +22,7 @@
 //
 // The tensor cores' fp32 accumulation is not an IEEE one: against fp64 the error of a sum of K products grows with K (measured,
 // random operands: 1e-6 of the result's norm at K = 1024, 4.4e-6 at 4096, 1.9e-5 at 16384).  fp32 results are therefore formed
-// in pieces of kGradChunk rows that the epilogue adds up, in order, in IEEE fp32 registers.  bf16 results round more than
+// in pieces of kGradChunk products that the epilogue adds up, in order, in IEEE fp32 registers.  bf16 results round more than
 // that away and take all rows in one piece, up to kGradOnePiece of them.
 //
 // Every wait is bounded; on a time-out status bit 1 is raised and all roles leave.
@@ -155,7 +155,7 @@ __device__ __forceinline__ void gg_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// ROWS = false: weight gradient, true: row product.  PIECES: sums in pieces of kGradChunk rows.  F32: results in fp32, else bf16.  WIDE:
+// ROWS = false: weight gradient, true: row product.  PIECES: sums in pieces of kGradChunk products.  F32: results in fp32, else bf16.  WIDE:
 // tiles of 256 x 512.  NA = 3: the sum is over three column ranges of A as well (the router's dlogits)
 template <bool ROWS, bool PIECES, bool F32, bool WIDE, int NA>
 __global__ void __launch_bounds__(GG_THREADS, 1)
@@ -241,7 +241,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   };
   auto steps_of = [&](const Item& w) { return (max(w.end - w.beg, 0) + GG_BK - 1) / GG_BK; };
   // K steps that one accumulator takes
-  auto piece = [&](int steps) { return PIECES ? kGradChunk / GG_BK : steps; };
+  auto piece = [&](int steps) { return PIECES ? kGradChunk / (GG_BK * NA) : steps; };
 
   if (MOVE_REGS && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GG_REG_LO));
   if (warp == 0) {
