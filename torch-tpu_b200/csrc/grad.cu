@@ -319,8 +319,12 @@ grad_finish_kernel(const FinishArgs a) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int64_t p = t * a.k + j0 + u;
-        on[u] = j0 + u < a.k && a.ids[p] >= 0 && a.ids[p] < a.E;  // (a dropped slot has no row)
-        if (on[u]) raw[u] = *reinterpret_cast<const uint4*>(a.y + p * a.H + c);
+        on[u] = j0 + u < a.k;
+        if (on[u]) {  // (a dropped slot's row was never written: it is loaded beside its id, not after it, and then left out)
+          raw[u] = *reinterpret_cast<const uint4*>(a.y + p * a.H + c);
+          const int id = a.ids[p];
+          on[u] = id >= 0 && id < a.E;
+        }
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
