@@ -270,10 +270,11 @@ def _chk_grad(t, name, dtypes, shape, device):
     raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _grad_out(t, name, dtypes, shape, device):
-    """`t`, checked, or a new tensor of the first of `dtypes`."""
+def _grad_out(t, name, dtypes, shape, like):
+    """`t`, checked, or a new tensor of the first of `dtypes`, on the device of `like`."""
+    device = like.device
     if t is None:
-        return torch.empty(shape, dtype=dtypes[0], device=device)
+        return like.new_empty(shape) if like.dtype is dtypes[0] else like.new_empty(shape, dtype=dtypes[0])
     _chk_grad(t, name, dtypes, shape, device)
     return t
 
@@ -296,7 +297,13 @@ _HERE = contextlib.nullcontext()
 
 
 def _raw_stream(device):
+    """The current stream's handle (asked for without making a Stream object of it, which takes a sixth of a small call)."""
+    if _handle_of_stream is not None:
+        return _handle_of_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_handle_of_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _workspace(workspace, need, what, device):
@@ -341,7 +348,7 @@ def route_backward(dw, logits, ids, score_func="softmax", renorm=True, scale=1.0
     if score_func not in ("softmax", "sigmoid"):
         raise ValueError(f"score_func must be softmax or sigmoid, got {score_func!r}")
     with _on(dev):
-        dlogits = _grad_out(dlogits, "dlogits", _F32, (T, E), dev)
+        dlogits = _grad_out(dlogits, "dlogits", _F32, (T, E), logits)
         sf = L.SCORE_SOFTMAX if score_func == "softmax" else L.SCORE_SIGMOID
         L.check(L.lib().b200moe_route_backward(_addr(dlogits), _addr(logits), _addr(logit_bias), _addr(ids), _addr(dw), _DT[dw.dtype],
                                                T, E, k, sf, int(renorm), float(scale), _raw_stream(dev)), "b200moe_route_backward")
@@ -370,8 +377,8 @@ def router_logits_backward(dlogits, x=None, wr=None, dx=None, dwr=None, accumula
     with _on(dev):
         need = L.lib().b200moe_router_logits_backward_workspace_bytes(T, H, E)
         keep, base, avail = _workspace(workspace, need, "b200moe_router_logits_backward", dev)
-        dx = _grad_out(dx, "dx", _BF16, (T, H), dev) if wr is not None else None
-        dwr = _grad_out(dwr, "dwr", _GRAD, (E, H), dev) if x is not None else None
+        dx = _grad_out(dx, "dx", _BF16, (T, H), wr) if wr is not None else None
+        dwr = _grad_out(dwr, "dwr", _GRAD, (E, H), dlogits) if x is not None else None
         L.check(L.lib().b200moe_router_logits_backward(_addr(dx), int(add_dx), _addr(dwr), _DT[dwr.dtype] if dwr is not None else L.F32,
                                                        int(accumulate and dwr is not None), _addr(dlogits), _addr(x), _addr(wr), T, H, E,
                                                        base, avail, _addr(status), _raw_stream(dev)), "b200moe_router_logits_backward")
@@ -390,8 +397,8 @@ def combine_backward(dout, y, w, ids=None, num_experts=0, dy=None, dw=None):
     if ids is not None:
         _chk_grad(ids, "ids", _I32, (T, k), dev)
     with _on(dev):
-        dy = _grad_out(dy, "dy", _BF16, (T, k, H), dev)
-        dw = _grad_out(dw, "dw", _F32, (T, k), dev)
+        dy = _grad_out(dy, "dy", _BF16, (T, k, H), y)
+        dw = _grad_out(dw, "dw", _F32, (T, k), y)
         L.check(L.lib().b200moe_combine_backward(_addr(dy), _addr(dw), _addr(dout), _addr(y), _addr(w), _DT[w.dtype], _addr(ids), num_experts,
                                                  T, k, H, _raw_stream(dev)), "b200moe_combine_backward")
     return dy, dw
@@ -418,8 +425,8 @@ def linear_w8_backward(dy, x=None, w=None, scale=None, dx=None, dw=None, accumul
         sdt = _DT[scale.dtype] if w is not None else L.F32
         need = L.lib().b200moe_linear_w8_backward_workspace_bytes(M, K, N, sdt)
         keep, base, avail = _workspace(workspace, need, "b200moe_linear_w8_backward", dev)
-        dx = _grad_out(dx, "dx", _BF16, (M, K), dev) if w is not None else None
-        dw = _grad_out(dw, "dw", _GRAD, (N, K), dev) if x is not None else None
+        dx = _grad_out(dx, "dx", _BF16, (M, K), dy) if w is not None else None
+        dw = _grad_out(dw, "dw", _GRAD, (N, K), dy) if x is not None else None
         L.check(L.lib().b200moe_linear_w8_backward(_addr(dx), _addr(dw), _DT[dw.dtype] if dw is not None else L.F32,
                                                    int(accumulate and dw is not None), _addr(dy), _addr(x), _addr(w),
                                                    _addr(scale) if w is not None else None, sdt, M, K, N, base, avail,
@@ -481,9 +488,9 @@ def experts_backward(dout, x, wg, wu, wd, sg, su, sd, ids, topk_w=None, *, dx=No
                                grad_dtype=weight_grads[0].dtype if weight_grads is not None else torch.float32,
                                accumulate=accumulate and weight_grads is not None)
         keep, base, avail = _workspace(workspace, experts_backward_workspace_bytes(d), "b200moe_experts_backward", dev)
-        dx = _grad_out(dx, "dx", _BF16, (T, H), dev)
+        dx = _grad_out(dx, "dx", _BF16, (T, H), x)
         if not per_slot:
-            dw = _grad_out(dw, "dw", _F32, (T, k), dev)
+            dw = _grad_out(dw, "dw", _F32, (T, k), x)
         g = [_addr(t) for t in weight_grads] if weight_grads is not None else [None] * 3
         L.check(L.lib().b200moe_experts_backward(_addr(dx), _addr(dw), *g, _addr(dout), _addr(x), _addr(wg), _addr(wu), _addr(wd), _addr(sg),
                                                  _addr(su), _addr(sd), _addr(ids), _addr(topk_w), _addr(add), ctypes.byref(d), base, avail,
