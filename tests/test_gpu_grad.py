@@ -362,3 +362,70 @@ def test_empty_batches(ops):
     ops.experts_backward(p["dout"], p["x"], *p["w"], *p["s"], p["ids"], p["topk_w"], weight_grads=[keep, keep.clone(), keep.clone()],
                          accumulate=True)
     assert bool((keep == 3.0).all())
+
+
+# ---- refusals with tensors on a GPU -----------------------------------------------------------------------------------
+def test_refusals(ops):
+    p = problem(8, 256, 128, 4, 2)
+    call = lambda q, **kw: ops.experts_backward(q["dout"], q["x"], *q["w"], *q["s"], q["ids"], q["topk_w"], **kw)  # noqa: E731
+    g32 = [torch.empty(w.shape, device=DEV) for w in p["w"]]
+    for match, q, kw in (
+        ("must have shape", {**p, "x": p["x"][:4]}, {}),
+        ("ids", {**p, "ids": p["ids"].long()}, {}),
+        ("contiguous", {**p, "x": p["x"].t().contiguous().t()}, {}),
+        ("wu", {**p, "w": [p["w"][0], p["w"][1][:2].contiguous(), p["w"][2]]}, {}),
+        ("wg", {**p, "w": [w.to(torch.bfloat16) for w in p["w"]]}, {}),              # bf16-weight experts
+        ("su", {**p, "s": [p["s"][0], p["s"][1].bfloat16(), p["s"][2]]}, {}),
+        ("topk_w", {**p, "topk_w": None}, {}),
+        ("topk_w", {**p, "topk_w": p["topk_w"].double()}, {}),
+        ("topk_w and dw", {**p, "dout": p["dout"][:, None].repeat(1, 2, 1)}, {}),
+        ("weight_grads", p, dict(weight_grads=g32[:2])),
+        ("one dtype", p, dict(weight_grads=[g32[0], g32[1].bfloat16(), g32[2]])),
+        ("accumulate", p, dict(weight_grads=[t.bfloat16() for t in g32], accumulate=True)),
+        ("dwd", p, dict(weight_grads=[g32[0], g32[1], None])),
+        ("add", p, dict(add=torch.zeros(8, 256, device=DEV))),
+        ("dx", p, dict(dx=torch.zeros(8, 128, dtype=torch.bfloat16, device=DEV))),
+        ("workspace", p, dict(workspace=torch.zeros(1 << 20, dtype=torch.uint8))),
+        ("status", p, dict(status=torch.zeros(1, dtype=torch.int32))),
+    ):
+        with pytest.raises(ValueError, match=match):
+            call(q, **kw)
+    with pytest.raises(RuntimeError, match="workspace"):
+        call(p, workspace=torch.zeros(4096, dtype=torch.uint8, device=DEV))
+    odd = torch.zeros(8 * 256 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(8, 256)      # not 16-byte aligned
+    with pytest.raises(RuntimeError, match="aligned"):
+        call({**p, "x": odd})
+    g = gen(1)
+    with pytest.raises(ValueError, match="unsupported sizes"):
+        ops.linear_w8_backward(randn(g, 4, 128), randn(g, 4, 100))
+    with pytest.raises(ValueError, match="unsupported sizes"):
+        ops.router_logits_backward(randn(g, 4, 8, dtype=torch.float32), randn(g, 4, 100))
+    with pytest.raises(ValueError, match="add_dx"):
+        ops.router_logits_backward(randn(g, 4, 8, dtype=torch.float32), None, randn(g, 8, 128), add_dx=True)
+    with pytest.raises(ValueError, match="scale"):
+        ops.linear_w8_backward(randn(g, 4, 128), None, fp8_weights(g, 1, 128, 128)[0][0])
+    with pytest.raises(RuntimeError, match="unsupported size"):
+        ops.combine_backward(randn(g, 4, 12), randn(g, 4, 2, 12), torch.ones(4, 2, device=DEV))
+    with pytest.raises(RuntimeError, match="unsupported size"):
+        ops.route_backward(torch.ones(2, 33, device=DEV), torch.zeros(2, 64, device=DEV), torch.zeros(2, 33, dtype=torch.int32, device=DEV))
+    with pytest.raises(ValueError, match="score_func"):
+        ops.route_backward(torch.ones(2, 2, device=DEV), torch.zeros(2, 64, device=DEV), torch.zeros(2, 2, dtype=torch.int32, device=DEV), "tanh")
+
+
+def test_non_finite_rows_stay_their_own(ops):
+    """A token whose row is not finite spoils what depends on it, and nothing else."""
+    T, E = 200, 6
+    p = problem(T, 256, 128, E, 2)
+    clean = run_experts(ops, p, torch.float32)
+    bad = 77
+    p["dout"][bad, 5] = float("nan")
+    p["x"][bad, 9] = float("inf")
+    dx, dw, grads, st = run_experts(ops, p, torch.float32)
+    keep = torch.arange(T, device=DEV) != bad
+    assert torch.isfinite(dx[keep]).all() and torch.isfinite(dw[keep]).all()
+    assert torch.equal(dw[keep], clean[1][keep])
+    assert not torch.isfinite(dx[bad]).all() and not torch.isfinite(dw[bad]).any()
+    mine = p["ids"][bad].long()
+    others = [e for e in range(E) if e not in mine.tolist()]
+    for t, c in zip(grads, clean[2]):
+        assert torch.equal(t[others], c[others]) and not torch.isfinite(t[mine]).all()

@@ -143,6 +143,28 @@ def test_layer_backward_replayed_from_a_graph():
     assert int(layer.status.item()) == 0
 
 
+def test_graph_outlives_a_larger_workspace():
+    """A graph captured without weight gradients is replayed after a call that needed a larger workspace."""
+    layer, x, dout, _ = make_layer(T=260, H=256, I=256, E=8, k=2)
+    layer.backward(x, dout)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = layer.backward(x, dout)
+    graph.replay()
+    want = res.dx.clone()
+    small = layer._bwd["workspace"]
+    layer.backward(x, dout, **grads_of(layer))
+    assert layer._bwd["workspace"].numel() > small.numel()
+    del small
+    torch.cuda.empty_cache()
+    fresh = [torch.full((1 << 20,), 255, dtype=torch.uint8, device=DEV) for _ in range(64)]   # takes what was given back
+    res.dx.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(res.dx, want) and all(bool((t == 255).all()) for t in fresh)
+
+
 def test_small_batch_replayed_from_a_graph():
     """dx of few pairs: a K range that is split, its partial sums cleared and added inside the graph."""
     layer, x, dout, _ = make_layer(T=12, H=512, I=1024, E=4, k=2)

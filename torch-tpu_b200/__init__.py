@@ -3,8 +3,8 @@ gate/up GEMM with SiLU-and-mul, down GEMM, weighted combine), written for NVIDIA
 behind the reference's own ``torch.ops.my_ops.*`` custom-op surface.
 
   lib      ctypes binding of the C ABI (include/b200moe.h)
-  ops      functional wrappers over the C ABI for torch CUDA tensors
-  layer    FusedMoE: route -> experts -> combine as one call, plus the expert-parallel variant
+  ops      functional wrappers over the C ABI for torch CUDA tensors, and the gradients of each (*_backward)
+  layer    FusedMoE: route -> experts -> combine as one call, its gradients (backward), plus the expert-parallel variant
   weights  checkpoint-layout -> op-layout conversion and FP8 block quantisation
   load_ops()  registers torch.ops.my_ops.{fused_moe_fused_experts, fused_moe_fused_experts_v2,
               fused_moe_grouped_topk, noaux_tc_topk, mlp_w8a16_dq_forward, mlp_w8a8_quant_forward}

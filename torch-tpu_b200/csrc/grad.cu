@@ -35,6 +35,7 @@ __device__ __forceinline__ float warp_max(float v) {
 //   softmax         dl_e = s_e * ((dp of the slots that chose e) - sum_i dp_i p_i)
 // Renormalised softmax weights depend on the selected logits alone (the last sum is zero): they are formed as a softmax
 // over those, so the row itself need not be read, and all other entries are exactly zero.
+// Bound by latency: 8192 tokens x 256 experts (8.4 MB written) 8.5 us from a cold cache, 16 x 8 in a graph 1.9.
 struct RouteGradArgs {
   float* dlogits;
   const float* logits;
@@ -112,7 +113,8 @@ route_grad_kernel(const RouteGradArgs a, int64_t T) {
 
 // ---- weighted combine -----------------------------------------------------------------------------------------------
 // dy[t,j,:] = w[t,j] * dout[t,:], dw[t,j] = <dout[t,:], y[t,j,:]>: one block per token, dout's row in registers (up to
-// CG_COLS columns at a time), the token's rows of y through it.  Bound by HBM: k rows in, k rows out.
+// CG_COLS columns at a time), the token's rows of y through it.  Bound by HBM: k rows in, k rows out (2048 tokens x 8 x 7168:
+// 87 us = 5.8 TB/s; one slot at a time 97).
 constexpr int CG_THREADS = 256;
 constexpr int CG_VEC = 4;                            // 16-byte pieces of a row per thread
 constexpr int CG_COLS = CG_THREADS * 8 * CG_VEC;     // 8192
@@ -184,6 +186,7 @@ combine_grad_kernel(__nv_bfloat16* dy, float* dw, const __nv_bfloat16* dout, con
 // Rows are read once: quantised (1 x 128, e4m3) and, where weight gradients are wanted, copied in bf16, both to the
 // positions of the row's slots (pos_of, -1 = dropped; NULL = row order).  A lane owns 16 consecutive columns, eight lanes
 // one 128-column group; a warp takes 512 columns of a row.  blockIdx.y: which of two tensors (tokens, gradients).
+// Bound by HBM: Mixtral shape, 4096 tokens, with copies, 268 MB in and out 47 us = 5.7 TB/s.
 struct PrepSide {
   const __nv_bfloat16* src;  // [rows, H]
   uint8_t* q;
@@ -252,7 +255,7 @@ int launch_prep(PrepArgs a, cudaStream_t st) {
 
 // ---- last step of the experts' gradient ------------------------------------------------------------------------------
 // dx[t,:] = sum over the token's slots of y[t*k+j,:] (or acc32[t,:]) (+ add[t,:]), in slot order; dw[t,j] = the partial sums
-// of the slot's row, in column order (0 for a dropped slot)
+// of the slot's row, in column order (0 for a dropped slot).  DeepSeek shape, 2048 tokens: 264 MB in 45 us = 5.9 TB/s.
 struct FinishArgs {
   __nv_bfloat16* dx;  // NULL = not wanted
   const __nv_bfloat16* y;
@@ -398,7 +401,7 @@ router_dwr_kernel(void* dwr, int f32, int add, const float* part, int parts, int
 
 // A few tokens: both products in one kernel on the CUDA cores.  A block owns 32 columns of H: the tokens' and the
 // router's columns and dlogits as fp32 in shared memory; a thread owns a column and every eighth token and expert.  fp32
-// sums in order.
+// sums in order.  16 tokens, 1024 x 8: 2.7 us in a graph; the four kernels of the general way 20.
 constexpr int RGS_COLS = 32, RGS_THREADS = 256, RGS_ROWS = RGS_THREADS / RGS_COLS;
 constexpr int RGS_MAX_T = 64, RGS_MAX_TE = 8192;  // tokens, tokens x experts
 __global__ void __launch_bounds__(RGS_THREADS)

@@ -137,6 +137,8 @@ class FusedMoE:
                 b.update(zeros=torch.zeros(n, 1, dtype=torch.int32, device=dev), ones=torch.ones(n, 1, device=dev),
                          shared_dw=torch.empty(n, 1, dtype=torch.float32, device=dev))
         if b["workspace"] is None or b["workspace"].numel() < max(need) + 256:
+            if b["workspace"] is not None:  # (a graph captured before this call still writes to the smaller one)
+                b.setdefault("kept", []).append(b["workspace"])
             b["workspace"] = torch.empty(max(need) + 256, dtype=torch.uint8, device=dev)
         return b
 

@@ -479,8 +479,10 @@ def experts_backward(dout, x, wg, wu, wd, sg, su, sd, ids, topk_w=None, *, dx=No
         if len(weight_grads) != 3:
             raise ValueError("weight_grads is (dwg, dwu, dwd)")
         for n, t in zip(("dwg", "dwu", "dwd"), weight_grads):
-            _chk_grad(t, n, (weight_grads[0].dtype,) if weight_grads[0].dtype in _GRAD else _GRAD, (E, I, H), dev)
+            _chk_grad(t, n, _GRAD, (E, I, H), dev)
             _chk_accumulate(accumulate, t, n)
+        if len({t.dtype for t in weight_grads}) > 1:
+            raise ValueError("dwg, dwu and dwd must be of one dtype")
     _chk_status(status, dev)
     with _on(dev):
         d = make_backward_desc(T, H, I, E, k, per_slot=per_slot, scale_dtype=sg.dtype,
