@@ -637,7 +637,7 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   a.P = (int)g.P;
   a.groups = g.groups, a.segs = g.segs;
   a.M = g.M, a.N = g.N;
-  const bool pieces = g.out_f32 || g.P > kGradOnePiece;
+  const bool pieces = g.out_f32 || g.rows > kGradOnePiece;
   a.MT = (g.M + 255) / 256;
   const bool wide = !pieces && gg_wide((int64_t)g.groups * g.segs * a.MT, g.N);
   a.NT = (g.N + (wide ? 511 : 255)) / (wide ? 512 : 256);

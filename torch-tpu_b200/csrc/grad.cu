@@ -561,7 +561,7 @@ extern "C" int b200moe_router_logits_backward(void* dx, int add_dx, void* dwr, i
     g.a = split;
     g.b0 = reinterpret_cast<const __nv_bfloat16*>(x);
     g.out[0] = part;
-    g.P = T;
+    g.P = g.rows = T;
     g.groups = L.parts, g.segs = 1, g.kparts = L.stacked ? 3 : 1, g.M = (L.stacked ? 1 : 3) * L.Ep, g.N = (int)H;
     g.out_f32 = 1;
     g.status = status;
@@ -671,7 +671,7 @@ extern "C" int b200moe_linear_w8_backward(void* dx, void* dw, int dw_dtype, int 
     g.a = reinterpret_cast<const __nv_bfloat16*>(dy);
     g.b0 = reinterpret_cast<const __nv_bfloat16*>(x);
     g.out[0] = dw;
-    g.P = M;
+    g.P = g.rows = M;
     g.groups = g.segs = g.kparts = 1, g.M = (int)N, g.N = (int)K;
     g.out_f32 = dw_dtype == B200MOE_F32, g.add = accumulate;
     g.status = status;
@@ -867,6 +867,7 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
     wg.out[0] = dw_gate, wg.out[1] = dw_up, wg.out[2] = dw_down;
     wg.offsets = I32(L.offsets);
     wg.P = L.P;
+    wg.rows = d->T;  // (a token takes an expert once)
     wg.groups = (int)d->E, wg.segs = 3, wg.kparts = 1, wg.M = (int)d->I, wg.N = (int)d->H;
     wg.out_f32 = d->grad_dtype == B200MOE_F32, wg.add = d->accumulate;
     wg.status = status;

@@ -145,6 +145,7 @@ struct MoeWeightGradArgs {
   void* out[3];
   const int32_t* offsets;
   int64_t P;
+  int64_t rows;                  // that a group has, hardly ever more
   int groups, segs, kparts, M, N;
   int out_f32, add;              // add: to what `out` holds (fp32 only)
   int32_t* status;
