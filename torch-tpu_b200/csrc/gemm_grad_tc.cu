@@ -10,7 +10,7 @@
 // columns, the leader issues MMAs of M256 N256 K16 that read both CTAs' shared memory, each CTA's tensor memory receives
 // its 128 rows.  One CTA alone moves 48 KB into shared memory and as much out of it per 512-cycle K step (M128 N256 K64), which
 // is more than the 128 bytes per cycle that shared memory has; a pair moves 32 KB per CTA.
-// 12 warps per CTA: warp 0 = TMA producer, warp 1 = MMA issuer (leader) and TMEM owner, warp 2 = tails, warps 4..11 = epilogue (lane quarter =
+// 12 warps per CTA: warp 0 = TMA producer, warp 1 = MMA issuer (leader) and TMEM owner, warp 2 = tails, warp 3 = groups without rows, warps 4..11 = epilogue (lane quarter =
 // warp % 4, column half = (warp - 4) / 4).  Five stages of 32 KB; two accumulators of 256 TMEM columns, so that the epilogue
 // of a tile runs beside the next tile's MMAs.  Results leave through swizzled shared-memory patches by TMA stores (or fp32
 // reductions), 32 rows x 128 bytes at a time.
@@ -81,7 +81,8 @@ constexpr size_t gg_smem_bytes() {
 static_assert(gg_smem_bytes<false, 1>() <= 232448 && gg_smem_bytes<true, 1>() <= 232448 && gg_smem_bytes<false, 3>() <= 232448, "more than the 227 KB of shared memory a CTA can have");
 
 struct GgArgs {
-  const int32_t* offsets;  // rows of group g: [offsets[g], offsets[g+1]); NULL = the `groups` even parts of [0, P)
+  const int4* order;       // the groups in the order in which they are worked on: {output, first row, end of its rows, -};
+                           // NULL = the `groups` even parts of [0, P)
   int P, groups, segs;     // segs: operand pairs that a group has (columns [seg * M, (seg + 1) * M) of A)
   int M, N, MT, NT;        // outputs of one (group, segment); tiles along both
   int out_rows;            // rows of the output between groups
@@ -229,9 +230,9 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     w.nt = r - w.mt * a.NT;
     if (ROWS) {
       w.beg = 0, w.end = a.K;
-    } else if (a.offsets) {
-      w.beg = a.offsets[w.g];
-      w.end = a.offsets[w.g + 1];
+    } else if (a.order) {
+      const int4 o = a.order[w.g];
+      w.g = o.x, w.beg = o.y, w.end = o.z;
     } else {  // whole K steps to each part
       const int64_t steps = (a.P + GG_BK - 1) / GG_BK;
       w.beg = (int)(steps * w.g / a.groups) * GG_BK;
@@ -374,6 +375,23 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       __syncwarp();
       if (lane == 0) gg_arrive(gg_in_cta(smem_u32(&sh->full[0]) + s * 8, 0));
     }
+  } else if (warp == 3 && !ROWS) {
+    // ------------------------------------------------------------------ experts without rows
+    // Zeros, where results are not added to what is there: plain stores beside the other roles' work, which goes on with the
+    // experts that have rows (those come first in the list, so both go on at once).
+    // The item's part of the expert's matrix, in 16-byte units, half to each CTA.
+    Item nx{};
+    if (pair0 < items) nx = item_of(pair0);
+    for (int t = pair0; t < items && !a.add; t += pairs) {
+      const Item w = fixed(nx);
+      if (t + pairs < items) nx = item_of(t + pairs);
+      if (w.beg < w.end) continue;
+      const int64_t units = (int64_t)a.M * a.N * (F32 ? 4 : 2) / 16, parts = (int64_t)a.MT * a.NT * 2;
+      const int64_t i = ((int64_t)w.mt * a.NT + w.nt) * 2 + rank, end = units * (i + 1) / parts;
+      uint4* out = reinterpret_cast<uint4*>(w.seg == 0 ? a.out0 : w.seg == 1 ? a.out1 : a.out2) + (int64_t)w.g * units;
+#pragma unroll 4
+      for (int64_t u = units * i / parts + lane; u < end; u += 32) out[u] = make_uint4(0, 0, 0, 0);
+    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue
     if (MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(GG_REG_HI));
@@ -381,12 +399,11 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     uint8_t* const patch0 = patches + (warp - 4) * (GG_PATCHES * GG_PATCH_BYTES);
     const uint32_t tmem_empty_leader = gg_in_cta(smem_u32(&sh->tmem_empty[0]), 0);
     uint32_t n = 0;
-    bool ok = true, zeros = false;  // zeros: the patches hold zeros (and stores may still read them)
-    // both patches, once the stores before have read them
+    bool ok = true;
+    // the warp's patches, once the stores before have read them
     auto take_patches = [&]() {
       if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
-      zeros = false;
       return reinterpret_cast<uint4*>(patch0);
     };
     auto patches_written = [&]() {
@@ -404,32 +421,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const int mrow = w.mt * 256 + rank * 128 + q * 32, row = w.g * a.out_rows + mrow, col0 = w.nt * Tile::NTILE + cg * 128;
       const bool rows_here = mrow < a.M;
       const int cols = rows_here ? min(128, a.N - col0) : 0;  // columns of this warp that exist (in the first 256)
-      if (w.beg >= w.end) {
-        // An expert without rows: zeros, not tile by tile but in runs (the 16 warps of the pair share the item's part of the
-        // expert's matrix, 16-byte units [u, end) each), straight from patches that are cleared once.
-        if (!a.add) {
-          if (!zeros) {
-            uint4* p = take_patches();
-#pragma unroll
-            for (int i = 0; i < GG_PATCHES * GG_PATCH_BYTES / 512; ++i) p[i * 32 + lane] = make_uint4(0, 0, 0, 0);
-            patches_written();
-            zeros = true;
-          }
-          if (lane == 0) {
-            const int64_t units = (int64_t)a.M * a.N * (F32 ? 4 : 2) / 16, parts = (int64_t)a.MT * a.NT * 2 * GG_EPI_WARPS;
-            const int64_t i = ((int64_t)w.mt * a.NT + w.nt) * 2 * GG_EPI_WARPS + rank * GG_EPI_WARPS + (warp - 4);
-            int64_t u = units * i / parts;
-            const int64_t end = units * (i + 1) / parts;
-            uint8_t* base = (w.seg == 0 ? a.out0 : w.seg == 1 ? a.out1 : a.out2) + (int64_t)w.g * units * 16;
-            for (; u < end; u += GG_PATCHES * GG_PATCH_BYTES / 16)
-              asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + u * 16), "r"(smem_u32(patch0)),
-                           "r"((uint32_t)(min(end - u, (int64_t)(GG_PATCHES * GG_PATCH_BYTES / 16)) * 16))
-                           : "memory");
-            sent();
-          }
-        }
-        continue;
-      }
+      if (w.beg >= w.end) continue;  // an expert without rows: warp 3's
       auto put = [&](uint4* p, int i, uint4 v) { p[lane * 8 + (i ^ (lane & 7))] = v; };  // the 128-byte swizzle
       const int steps = steps_of(w), per = piece(steps);
       auto release = [&](uint32_t buf) {  // the accumulator is in registers (or nobody wants it)
@@ -625,7 +617,7 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   CUtensorMap tm[6];
   if (g.M % 64) return B200MOE_ESHAPE;
   // (three ranges: no tails, their ends are ends of the tensor or of whole steps)
-  if (g.kparts != 1 && !(g.kparts == 3 && g.segs == 1 && !g.offsets && g.out_f32)) return B200MOE_EINVAL;
+  if (g.kparts != 1 && !(g.kparts == 3 && g.segs == 1 && !g.order && g.out_f32)) return B200MOE_EINVAL;
   const int64_t acols = (int64_t)g.segs * g.M * g.kparts;
   if (!gg_make_chunk_map(&tm[0], g.a, (uint64_t)g.P, (uint64_t)acols)) return B200MOE_EDRIVER;
   if (!gg_make_b_map(&tm[1], g.b0, (uint64_t)g.P, (uint64_t)g.N)) return B200MOE_EDRIVER;
@@ -633,7 +625,7 @@ int moe_weight_grad_tc(const MoeWeightGradArgs& g, cudaStream_t st) {
   for (int i = 0; i < 3; ++i)
     if (!gg_make_map(&tm[3 + i], g.out[i < g.segs ? i : 0], g.out_f32, (uint64_t)g.groups * g.M, (uint64_t)g.N, 32)) return B200MOE_EDRIVER;
   GgArgs a{};
-  a.offsets = g.offsets;
+  a.order = g.order;
   a.P = (int)g.P;
   a.groups = g.groups, a.segs = g.segs;
   a.M = g.M, a.N = g.N;

@@ -136,14 +136,14 @@ int moe_gemm2_w8a16_tc(const MoeGemmArgs& a, cudaStream_t st);
 int moe_gather_rows_bf16(__nv_bfloat16* dst, const __nv_bfloat16* x, const int32_t* row_map, int div, int64_t rows,
                          int H, cudaStream_t st);
 // weight gradients on the tensor cores (gemm_grad_tc.cu): out[seg][g * M + m, n] (+)= sum of a[r, seg * M + m] * b[r, n] over the
-// rows r of group g, b = b1 for segment 2, else b0.  Groups are [offsets[g], offsets[g+1]), clipped to P, or (offsets NULL) the
-// even parts of [0, P).  With kparts > 1 (one segment, no offsets) a has kparts * M columns and the sum is over those of every part
+// rows r of group g, b = b1 for segment 2, else b0.  Groups come from a list, clipped to P (worked on in its order), or (order NULL) are the
+// even parts of [0, P).  With kparts > 1 (one segment, no list) a has kparts * M columns and the sum is over those of every part
 // too.  M % 64 == 0, with several segments M % 128 == 0; N % 8 == 0
 struct MoeWeightGradArgs {
   const __nv_bfloat16* a;        // [P, segs * kparts * M]
   const __nv_bfloat16 *b0, *b1;  // [P, N]
   void* out[3];
-  const int32_t* offsets;
+  const int4* order;             // per group {output, first row, end of its rows, -}, or NULL
   int64_t P;
   int64_t rows;                  // that a group has, hardly ever more
   int groups, segs, kparts, M, N;

@@ -97,7 +97,8 @@ class FusedMoE:
         shared expert, leading dim 1) are buffers that receive the weights' gradients; what is None is not formed.
         ``accumulate`` adds to what they hold (fp32).  Views of internal buffers are returned, unless ``dx`` is given, and
         hold until the next call.  Allocates on the first call of a kind only; can be captured into a CUDA graph after it.
-        FP8 weights and W8A8 arithmetic only.  Not an autograd function: the caller chains it, last layer first."""
+        FP8 weights and W8A8 arithmetic only, on one GPU (the expert-parallel layers have no gradient).  Not an autograd
+        function: the caller chains it, last layer first."""
         T, H = x.shape
         c = self.cfg
         if T > self.max_tokens:
