@@ -275,7 +275,7 @@ int b200moe_scaled_mm(void* out, int out_dtype, const void* a, const void* b, co
  * reference counterpart (its MoE ops are inference ops).  Products with FP8 weights run on the FP8 tensor cores as in the
  * forward call: Q(.) below quantises rows to e4m3 per 128 columns, scale = max|.| / 448 (the maximum is taken as at least 1e-12
  * for activations and 1e-30 for gradients), and gradients pass a quantisation unchanged.  Sums are fp32.  Equal calls give
- * equal bits, except dx of b200moe_experts_backward at T*k <= 512 (partial sums may meet in fp32 reductions there).
+ * equal bits.
  * Weight gradients are in the weights' layout, fp32 or bf16 (`*_dtype`); accumulate = 1 (fp32 only) adds them to what
  * the buffer holds.  Experts without rows get a zero gradient.  With T = 0 only the weight gradients are written (zeros).
  * Tensors may not overlap unless a call says so. */
@@ -315,8 +315,8 @@ int b200moe_linear_w8_backward(void* dx, void* dw, int dw_dtype, int accumulate,
  *   g = Q(x) Wg^T, u = Q(x) Wu^T, h = silu(g) * u          (formed again: nothing of the forward call is kept)
  *   d = Q(dout) Wd                                         (Wd: the down projection, stored as w_down [I,H])
  *   dw[t,j] = <h, d>;  dg = w d u silu'(g),  du = w d silu(g)
- *   dx[t,:] = sum_j (Q(dg) Wg + Q(du) Wu) (+ add[t,:])      (a slot's row is rounded to bf16 before the
- *                                                          sum, unless T*k <= 512 and K is split)
+ *   dx[t,:] = sum_j (Q(dg) Wg + Q(du) Wu) (+ add[t,:])      (a slot's row may be rounded to bf16 before
+ *                                                          the sum)
  *   dWg = sum dg^T x,  dWu = sum du^T x,  dWd = sum (w h)^T dout   over the expert's rows; dg, du and w h rounded to bf16
  *   dx        bf16 [T,H] or NULL           dw  fp32 [T,k] or NULL (NULL with per_slot)
  *   dw_gate, dw_up, dw_down  [E,I,H] of grad_dtype (weight_grads = 1; else ignored)

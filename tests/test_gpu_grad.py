@@ -273,7 +273,8 @@ def check_experts(ops, p, grad_dtype, bad=False, add=None):
 
 
 @pytest.mark.parametrize("T,H,I,E,k", [(1, 128, 128, 1, 1), (1, 256, 384, 8, 2), (16, 1024, 512, 8, 2), (37, 640, 128, 5, 3), (130, 128, 256, 4, 2),
-                                       (300, 384, 256, 6, 3), (700, 256, 128, 64, 4), (64, 256, 128, 200, 8)])
+                                       (300, 384, 256, 6, 3), (700, 256, 128, 64, 4), (64, 256, 128, 200, 8),
+                                       (1, 512, 2048, 4, 2), (30, 256, 1024, 8, 2), (33, 384, 1024, 3, 2)])
 @pytest.mark.parametrize("grad_dtype", [None, torch.bfloat16, torch.float32])
 def test_experts_backward(ops, T, H, I, E, k, grad_dtype):
     check_experts(ops, problem(T, H, I, E, k), grad_dtype)
@@ -297,12 +298,12 @@ def test_experts_backward_uneven_loads(ops):
     check_experts(ops, problem(70, 128, 128, 3, 2, ids=torch.full((70, 2), 2)), torch.bfloat16)  # the same expert twice
 
 
-@pytest.mark.parametrize("T", [20, 400])
-def test_experts_backward_dropped_pairs(ops, T):
+@pytest.mark.parametrize("T,I", [(20, 1024), (20, 128), (400, 128)])
+def test_experts_backward_dropped_pairs(ops, T, I):
     g = torch.Generator().manual_seed(T)
     ids = torch.randint(-1, 8, (T, 3), generator=g)          # -1, 6 and 7 are nobody's
     ids[3] = -1
-    p = problem(T, 256, 128, 6, 3, ids=ids)
+    p = problem(T, 256, I, 6, 3, ids=ids)
     dx, dw, grads, st = run_experts(ops, p, torch.float32)
     assert st == 1
     on = (p["ids"] >= 0) & (p["ids"] < 6)
@@ -331,11 +332,12 @@ def test_experts_backward_add_and_accumulate(ops, T):
         assert torch.equal(a, b + t)                          # one fp32 addition to each element
 
 
-def test_experts_backward_repeats_and_leaves_nothing_behind(ops):
-    """Equal calls give equal bits above 512 pairs; a workspace full of NaN changes nothing."""
+@pytest.mark.parametrize("T,I", [(1, 1024), (20, 1024), (100, 512), (500, 256)])
+def test_experts_backward_repeats_and_leaves_nothing_behind(ops, T, I):
+    """Equal calls give equal bits; a workspace full of NaN changes nothing."""
     import torch_tpu_b200
-    p = problem(500, 256, 256, 16, 2)
-    d = ops.make_backward_desc(500, 256, 256, 16, 2, weight_grads=True, grad_dtype=torch.bfloat16)
+    p = problem(T, 256, I, 16, 2)
+    d = ops.make_backward_desc(T, 256, I, 16, 2, weight_grads=True, grad_dtype=torch.bfloat16)
     ws = torch.full((ops.experts_backward_workspace_bytes(d) + 256,), 255, dtype=torch.uint8, device=DEV)
     first = run_experts(ops, p, torch.bfloat16, workspace=ws)
     for _ in range(3):

@@ -278,6 +278,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const int nIs = (a.I + kBlock - 1) / kBlock;  // scale rows of one expert (= nI unless a linear layer's N % 128 != 0)
   struct Item {
     int nt, mt, kb0, KB;
+    int ks;  // (MODE 4) the K split
   };
   auto item_of = [&](int t) {
     Item w;
@@ -288,6 +289,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     } else {
       ks = t % a.KS, tt = t / a.KS;
     }
+    if (MODE == 4) w.ks = ks;
     w.nt = a.m_major ? tt % a.NT : tt / num_mtiles;
     w.mt = a.m_major ? tt / a.NT : tt - w.nt * num_mtiles;
     if (!GATE_UP && a.part) return w;
@@ -442,7 +444,7 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       if (lane == 0) {
         sh->head_item[0] = e, sh->head_item[1] = row0, sh->head_item[2] = row_end;
         sh->head_item[3] = w.nt, sh->head_item[4] = w.kb0, sh->head_item[5] = w.KB;
-        if (MODE == 3 || MODE == 5) sh->head_item[6] = w.mt;
+        if (MODE >= 3) sh->head_item[6] = MODE == 4 ? w.ks : w.mt;
       }
       if (lane < 4) sh->head_w[lane] = wv;
 #pragma unroll
@@ -526,14 +528,14 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     for (int t = blockIdx.x; t < total_tiles; t += gridDim.x, ++ntile) {
       // the item (its integer divisions included), its expert and rows and the scales of its first two K blocks: left
       // in shared memory by the scout warp
-      Item w{0, 0, 0, 0};
+      Item w{0, 0, 0, 0, 0};
       int e = 0, row0 = 0, row_end = 0;
       float f0 = 0.f, f1 = 0.f, sa1 = 0.f, wa1 = 0.f, wb1 = 0.f;
       if (!mbar_wait(smem_u32(&sh->head_full), ntile & 1, abort_flag)) ok = false;
       if (ok) {
         e = sh->head_item[0], row0 = sh->head_item[1], row_end = sh->head_item[2];
         w.nt = sh->head_item[3], w.kb0 = sh->head_item[4], w.KB = sh->head_item[5];
-        if (MODE == 3 || MODE == 5) w.mt = sh->head_item[6];
+        if (MODE >= 3) (MODE == 4 ? w.ks : w.mt) = sh->head_item[6];
         // Scale factors f0 = sa[row,kb] * sw_gate[kb], f1 = sa[row,kb] * sw_up[kb]: the products of block kb + 1 are
         // formed and the values of block kb + 2 are requested while block kb's TMEM loads are in flight.
         const float sa0 = sh->head_sa[0][rit];
@@ -980,7 +982,14 @@ moe_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int col = nt * 256 + j * 128 + cg * TC_CW;
-          if (col < OUTW && a.KS > 1) {  // K split: partial sums meet in the fp32 buffer
+          if (MODE == 4 && col < OUTW) {  // K split: every part has rows of its own, [KS][P, H]
+            float4* dst = reinterpret_cast<float4*>(a.out32 + ((int64_t)w.ks * a.P + dstrow) * OUTW + col);
+#pragma unroll
+            for (int v4 = 0; v4 < TC_CW / 4; ++v4) {
+              const float2 p0 = unpack2(acc[j][v4 * 2]), p1 = unpack2(acc[j][v4 * 2 + 1]);
+              dst[v4] = make_float4(p0.x, p0.y, p1.x, p1.y);
+            }
+          } else if (col < OUTW && a.KS > 1) {  // K split: partial sums meet in the fp32 buffer
             float* dst32 = a.out32 + dstrow * OUTW + col;
 #pragma unroll
             for (int v4 = 0; v4 < TC_CW / 4; ++v4) {

@@ -280,12 +280,13 @@ int launch_prep(PrepArgs a, cudaStream_t st) {
 }
 
 // ---- last step of the experts' gradient ------------------------------------------------------------------------------
-// dx[t,:] = sum over the token's slots of y[t*k+j,:] (or acc32[t,:]) (+ add[t,:]), in slot order; dw[t,j] = the partial sums
+// dx[t,:] = sum over the token's slots of y[t*k+j,:] (or of its parts) (+ add[t,:]), in slot order; dw[t,j] = the partial sums
 // of the slot's row, in column order (0 for a dropped slot).  DeepSeek shape, 2048 tokens: 264 MB in 45 us = 5.9 TB/s.
 struct FinishArgs {
   __nv_bfloat16* dx;  // NULL = not wanted
   const __nv_bfloat16* y;
-  const float* acc32;
+  const float* slabs;  // instead of y: [slab_parts][T * k, H], the parts of every row's sum
+  int slab_parts;
   const __nv_bfloat16* add;
   const int32_t* ids;
   float* dw;          // NULL = not wanted
@@ -335,11 +336,28 @@ grad_finish_kernel(const FinishArgs a) {
       acc[2 * i] += f.x, acc[2 * i + 1] += f.y;
     }
   };
-  if (a.acc32) {
+  if (a.slabs) {
+    // (slot by slot, part by part; eight rows' pieces are on the way at a time, a dropped slot's among them)
+    const int n = a.k * a.slab_parts;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float4 lo[8], hi[8];
+      bool on[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(a.acc32 + t * a.H + c + i * 4);
-      acc[4 * i] = v.x, acc[4 * i + 1] = v.y, acc[4 * i + 2] = v.z, acc[4 * i + 3] = v.w;
+      for (int u = 0; u < 8; ++u) {
+        on[u] = i0 + u < n;
+        if (!on[u]) continue;
+        const int64_t p = t * a.k + (i0 + u) / a.slab_parts;
+        const float4* v = reinterpret_cast<const float4*>(a.slabs + ((i0 + u) % a.slab_parts * a.T * a.k + p) * a.H + c);
+        lo[u] = v[0], hi[u] = v[1];
+        const int id = a.ids[p];
+        on[u] = id >= 0 && id < a.E;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (!on[u]) continue;
+        acc[0] += lo[u].x, acc[1] += lo[u].y, acc[2] += lo[u].z, acc[3] += lo[u].w;
+        acc[4] += hi[u].x, acc[5] += hi[u].y, acc[6] += hi[u].z, acc[7] += hi[u].w;
+      }
     }
   } else {
     for (int j0 = 0; j0 < a.k; j0 += 4) {
@@ -605,10 +623,33 @@ extern "C" int b200moe_router_logits_backward(void* dx, int add_dx, void* dwr, i
 // ---- linear layer -----------------------------------------------------------------------------------------------------
 namespace {
 struct LinGradLayout {
-  size_t offsets, mtiles, nmt, q, s, sc32, part, cnt, y32, total;
+  size_t offsets, mtiles, nmt, q, s, sc32, part, cnt, total;
   int64_t ld;
-  int max_mtiles;
+  int max_mtiles, ksplit;
 };
+// One row of tiles leaves most SMs without one, so the K range (N) is cut: every part's sums go to rows of their own and a kernel adds the
+// parts up in K order.  The GEMM's own shared tiles, which a last CTA finishes, spend 14 of 30 thousand cycles on that with 16 rows.
+// Rows of their own / shared tiles, us in a graph: 6144 x 4096, 16 rows 15.5 / 22.4, 64 rows 18.7 / 23.4; 1024 x 4096, 64 rows 12.3 / 11.7,
+// 128 rows 16.3 / 11.9 (a thread's stores go to its row, so they grow with the rows); 8192 x 7168, 1 row 18.8 / 27.9.
+constexpr int64_t kSlabRows = 64;
+int lin_grad_ksplit(int64_t K, int64_t N) {
+  const int64_t tiles = (K + 255) / 256, blocks = (N + kBlock - 1) / kBlock;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(148 / tiles, blocks / 4));  // (by the sizes alone, whatever device runs)
+}
+__global__ void __launch_bounds__(256)
+slab_sum_kernel(__nv_bfloat16* out, const float* slabs, int parts, int64_t n) {
+  pdl_begin();
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) {
+    const float4 v = *reinterpret_cast<const float4*>(slabs + p * n + i);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(s.x, s.y), __floats2bfloat162_rn(s.z, s.w)};
+  *reinterpret_cast<uint2*>(out + i) = *reinterpret_cast<const uint2*>(b);
+}
 LinGradLayout lin_grad_layout(int64_t M, int64_t K, int64_t N, int scale_dtype) {
   LinGradLayout L{};
   Carve w;
@@ -621,7 +662,10 @@ LinGradLayout lin_grad_layout(int64_t M, int64_t K, int64_t N, int scale_dtype) 
   L.q = w.take((size_t)L.ld * N);
   L.s = w.take((size_t)nN * L.ld * sizeof(float));
   L.sc32 = w.take(scale_dtype == B200MOE_BF16 ? (size_t)nN * (K / kBlock) * sizeof(float) : 0);
-  L.part = w.take(moe_split_part_bytes(M));
+  // partial sums: of shared tiles, or of a cut K range (for min(M, limit) rows whatever M is: never smaller for more rows)
+  const int ks = lin_grad_ksplit(K, N);
+  L.ksplit = M <= kSlabRows && ks > 1 ? ks : 1;
+  L.part = w.take(std::max(moe_split_part_bytes(M), ks > 1 ? (size_t)ks * std::min<int64_t>(M, kSlabRows) * K * sizeof(float) : 0));
   L.cnt = w.take(kSplitCounters * sizeof(int32_t));
   L.total = w.total;
   return L;
@@ -686,10 +730,14 @@ extern "C" int b200moe_linear_w8_backward(void* dx, void* dw, int dw_dtype, int 
     g.I = (int)N;
     g.E = 1;
     g.segs = 1;
-    g.split = MoeSplitBuffers{reinterpret_cast<float*>(ws + L.part), I32(L.cnt)};
+    float* part = reinterpret_cast<float*>(ws + L.part);
+    if (L.ksplit > 1) g.ksplit = L.ksplit, g.out32 = part;
+    else g.split = MoeSplitBuffers{part, I32(L.cnt)};
     g.out = reinterpret_cast<__nv_bfloat16*>(dx);
     g.status = status;
     rc = moe_dx_tc(g, st);
+    if (!rc && L.ksplit > 1)
+      rc = moe_launch(slab_sum_kernel, (unsigned)((M * K / 4 + 255) / 256), 256, 0, st, g.out, part, L.ksplit, M * K);
     if (rc) return rc;
   }
   if (dw) {
@@ -708,6 +756,12 @@ extern "C" int b200moe_linear_w8_backward(void* dx, void* dw, int dw_dtype, int 
 
 // ---- experts ------------------------------------------------------------------------------------------------------------
 namespace {
+// dx of few pairs whose tiles leave half of the SMs without one: its K range is split, every part has rows of its own and the last step adds
+// them up in order.  Otherwise tiles are shared (schedule.h), which repeats to the bit as well.  dx and dw, us in a graph: sums in
+// order by this rule / parts that meet in fp32 reductions, as in the forward pass's down GEMM: small layer, 32 pairs 36.9 / 35.0; Mixtral
+// shape, 2 pairs 151 / 138, 32 pairs 459 / 460, 512 pairs 528 / 514; Qwen3 shape, 8 pairs 48.6 / 44.4, 512 pairs 237 / 237.
+constexpr int64_t kSlabPairs = 64;
+constexpr int kMaxKSplit = 16;  // of moe_choose_ksplit
 struct ExpGradLayout {
   size_t offsets, sorted, pos_of, scratch, mtiles, nmt, cnt, xq, xs, dq, ds, dh, gq, gs, dwp, y, shared, sc32, x16, d16, g16, order, total;
   int64_t P, ld;
@@ -720,7 +774,8 @@ ExpGradLayout exp_grad_layout(const b200moe_experts_backward_desc& d) {
   L.P = P;
   L.ld = (int64_t)align_up((size_t)P, kTileM);
   L.max_mtiles = (int)(P / kTileM + std::min(d.E, P));  // (an expert with rows has less than one tile more than they fill)
-  L.ksplit = moe_choose_ksplit(P, d.E, d.H, 2 * d.I);
+  L.ksplit = P <= kSlabPairs && 2 * std::min(d.E, P) * ((d.H + 255) / 256) <= 148
+                 ? std::min(moe_choose_ksplit(P, d.E, d.H, 2 * d.I), kMaxKSplit) : 1;
   L.offsets = w.take((d.E + 1) * sizeof(int32_t));
   L.sorted = w.take((size_t)P * sizeof(int32_t));
   L.pos_of = w.take((size_t)P * sizeof(int32_t));
@@ -737,9 +792,9 @@ ExpGradLayout exp_grad_layout(const b200moe_experts_backward_desc& d) {
   L.gs = w.take((size_t)2 * nI * L.ld * sizeof(float));
   L.dwp = w.take(d.per_slot ? 0 : (size_t)2 * nI * L.ld * sizeof(float));
   L.y = w.take((size_t)P * d.H * 2);
-  // partial sums of shared tiles, or the fp32 rows that a split K range of dx adds into (small batches): never both in one launch
-  // (for min(P, limit) rows whatever P is, so that the workspace size never shrinks when T grows)
-  L.shared = w.take(std::max(moe_split_part_bytes(P), (size_t)std::min<int64_t>(P, 512) * d.H * sizeof(float)));
+  // partial sums of shared tiles, or of a split K range of dx: never both in one launch (for min(P, limit) rows whatever P is, so that the
+  // workspace size never shrinks when T grows)
+  L.shared = w.take(std::max(moe_split_part_bytes(P), (size_t)kMaxKSplit * std::min<int64_t>(P, kSlabPairs) * d.H * sizeof(float)));
   L.sc32 = w.take(d.scale_dtype == B200MOE_BF16 ? 3 * (size_t)d.E * nI * nH * sizeof(float) : 0);
   if (d.weight_grads) {
     L.order = w.take((size_t)d.E * sizeof(int4));
@@ -802,7 +857,7 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
   auto F32 = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
   auto U8 = [&](size_t off) { return reinterpret_cast<uint8_t*>(ws + off); };
   auto B16 = [&](size_t off) { return reinterpret_cast<__nv_bfloat16*>(ws + off); };
-  const bool fused = L.ksplit > 1 && dx;  // dx's partial sums meet in fp32 rows
+  const bool slabs = L.ksplit > 1 && dx;
 
   rc = moe_permute_impl(I32(L.sorted), I32(L.offsets), ids, d->T, d->k, d->E, I32(L.scratch), status, I32(L.pos_of), I32(L.mtiles),
                         I32(L.nmt), L.max_mtiles, I32(L.cnt), stream);
@@ -869,21 +924,15 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
   rc = moe_swiglu_grad_tc(s, st);
   if (rc) return rc;
 
-  float* acc32 = F32(L.shared);
   if (dx) {
     MoeGemmArgs y = s;
     y.aq = s.hq;
     y.as_t = s.hs_t;
     y.segs = 2;
     y.comb_w = nullptr;
-    y.split = g.split;
     y.out = B16(L.y);
-    if (fused) {
-      const cudaError_t e = cudaMemsetAsync(acc32, 0, (size_t)d->T * d->H * sizeof(float), st);
-      if (e != cudaSuccess) return (int)e;
-      y.comb32 = acc32;
-      y.ksplit = L.ksplit;
-    }
+    if (slabs) y.out32 = F32(L.shared), y.ksplit = L.ksplit;
+    else y.split = g.split;
     rc = moe_dx_tc(y, st);
     if (rc) return rc;
   }
@@ -906,7 +955,8 @@ extern "C" int b200moe_experts_backward(void* dx, float* dw, void* dw_gate, void
     FinishArgs f{};
     f.dx = reinterpret_cast<__nv_bfloat16*>(dx);
     f.y = B16(L.y);
-    f.acc32 = fused ? acc32 : nullptr;
+    f.slabs = slabs ? F32(L.shared) : nullptr;
+    f.slab_parts = L.ksplit;
     f.add = reinterpret_cast<const __nv_bfloat16*>(add);
     f.ids = ids;
     f.dw = dw;
