@@ -104,6 +104,52 @@ def test_layer_backward_refuses():
         layer.backward(x, dout)
 
 
+def test_layer_backward_refuses_dx_over_its_inputs():
+    layer, x, dout, _ = make_layer(T=8, H=128, I=128, E=4, k=2, shared=128)
+    with pytest.raises(ValueError, match="shares memory with x"):
+        layer.backward(x, dout, dx=x)
+    with pytest.raises(ValueError, match="shares memory with dout"):
+        layer.backward(x, dout, dx=dout)
+    got = layer.backward(x, dout)
+    with pytest.raises(ValueError, match="shares memory with dout"):     # the returned view is the next call's dx
+        layer.backward(x, got.dx)
+    layer.backward(x, got.dx.clone())
+
+
+@pytest.mark.parametrize("bad", ["router type", "router shape", "shared type", "shared count"])
+def test_refused_call_adds_nothing(bad):
+    """accumulate with one unfit buffer: the others keep what they hold."""
+    layer, x, dout, _ = make_layer(T=8, H=128, I=128, E=4, k=2, shared=128)
+    kw = grads_of(layer, fill=1.0)
+    if bad == "router type":
+        kw["router_grad"] = kw["router_grad"].bfloat16()
+    elif bad == "router shape":
+        kw["router_grad"] = kw["router_grad"][:3]
+    elif bad == "shared type":
+        kw["shared_grads"][2] = kw["shared_grads"][2].bfloat16()
+    else:
+        kw["shared_grads"] = kw["shared_grads"][:2]
+    with pytest.raises(ValueError):
+        layer.backward(x, dout, accumulate=True, **kw)
+    torch.cuda.synchronize()
+    assert all(bool((t == 1).all()) for t in (kw["router_grad"], *kw["weight_grads"], *kw["shared_grads"]))
+
+
+def test_first_call_inside_a_capture_is_refused():
+    layer, x, dout, _ = make_layer(T=8, H=128, I=128, E=4, k=2, shared=128)
+    warm, _, _, _ = make_layer(T=8, H=128, I=128, E=4, k=2, shared=128)
+    want = warm.backward(x, dout)                                        # (kernel attributes are set; `layer` has no buffers yet)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(0)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            layer.backward(x, dout)
+    assert not layer._bwd
+    got = layer.backward(x, dout)                                        # same weights: the same generator
+    assert torch.equal(got.dx, want.dx) and torch.equal(got.dlogits, want.dlogits)
+
+
 def test_layer_backward_smaller_batches_and_empty():
     """One layer, one workspace, batches of any size up to max_tokens, in any order."""
     layer, x, dout, _ = make_layer(T=600, H=256, I=256, E=8, k=2, shared=128)

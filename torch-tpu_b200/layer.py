@@ -96,7 +96,8 @@ class FusedMoE:
         ``router_grad`` [E,H] fp32 or bf16, ``weight_grads`` = (dwg, dwu, dwd) [E,I,H] and ``shared_grads`` (the same for the
         shared expert, leading dim 1) are buffers that receive the weights' gradients; what is None is not formed.
         ``accumulate`` adds to what they hold (fp32).  Views of internal buffers are returned, unless ``dx`` is given, and
-        hold until the next call.  Allocates on the first call of a kind only; can be captured into a CUDA graph after it.
+        hold until the next call (which can therefore not take the returned dx as its x or dout).  Allocates on the first call
+        of a kind only; can be captured into a CUDA graph after it, not before.
         FP8 weights and W8A8 arithmetic only, on one GPU (the expert-parallel layers have no gradient).  Not an autograd
         function: the caller chains it, last layer first."""
         T, H = x.shape
@@ -107,9 +108,20 @@ class FusedMoE:
             raise ValueError("the gradient is that of FP8 weights in W8A8 arithmetic")
         if shared_grads is not None and self.shared is None:
             raise ValueError("shared_grads without a shared expert")
+        # (here, not in the calls below: nothing has been added to a buffer when another one is refused)
+        if router_grad is not None:
+            ops.check_weight_grads([router_grad], ["router_grad"], self.router_w.shape, accumulate, self.device)
+        for grads, weights, name in ((weight_grads, self.w, "weight_grads"), (shared_grads, self.shared, "shared_grads")):
+            if grads is not None:
+                if len(grads) != 3:
+                    raise ValueError(f"{name} is (dwg, dwu, dwd)")
+                ops.check_weight_grads(grads, [f"{name}[{i}]" for i in range(3)], weights[0].shape, accumulate, self.device)
         b = self._backward_buffers(weight_grads is not None, shared_grads is not None)
-        ids, w = self.route(x) if T else (self.ids[:0], self.topk_w[:0])
         dx = b["dx"][:T] if dx is None else dx
+        for n, t in (("x", x), ("dout", dout)):  # (both are read after dx's first store)
+            if ops.overlap(dx, t):
+                raise ValueError(f"dx shares memory with {n}")
+        ids, w = self.route(x) if T else (self.ids[:0], self.topk_w[:0])
         if self.shared is not None:  # the shared expert is one expert that every token takes with weight 1
             ops.experts_backward(dout, x, *self.shared, b["zeros"][:T], b["ones"][:T], dx=dx, dw=b["shared_dw"][:T],
                                  weight_grads=shared_grads, accumulate=accumulate, workspace=b["workspace"], status=self.status)
@@ -130,17 +142,21 @@ class FusedMoE:
         if self.shared is not None:
             need.append(ops.experts_backward_workspace_bytes(ops.make_backward_desc(
                 n, c.hidden, c.shared_intermediate, 1, 1, scale_dtype=self.shared[3].dtype, weight_grads=shared_grads)))
-        if not b:
+        old = b.get("workspace")
+        if old is not None and old.numel() >= max(need) + 256:
+            return b
+        if torch.cuda.is_current_stream_capturing():  # the buffers would be the graph's, and their first values written by its replays alone
+            raise RuntimeError("a first call of this kind allocates: make one before the capture")
+        if old is None:
             b.update(dx=torch.empty(n, c.hidden, dtype=torch.bfloat16, device=dev),
                      dw=torch.empty(n, c.top_k, dtype=torch.float32, device=dev),
-                     dlogits=torch.empty(n, c.num_experts, dtype=torch.float32, device=dev), workspace=None)
+                     dlogits=torch.empty(n, c.num_experts, dtype=torch.float32, device=dev))
             if self.shared is not None:
                 b.update(zeros=torch.zeros(n, 1, dtype=torch.int32, device=dev), ones=torch.ones(n, 1, device=dev),
                          shared_dw=torch.empty(n, 1, dtype=torch.float32, device=dev))
-        if b["workspace"] is None or b["workspace"].numel() < max(need) + 256:
-            if b["workspace"] is not None:  # (a graph captured before this call still writes to the smaller one)
-                b.setdefault("kept", []).append(b["workspace"])
-            b["workspace"] = torch.empty(max(need) + 256, dtype=torch.uint8, device=dev)
+        else:  # (a graph captured before this call still writes to the smaller one)
+            b.setdefault("kept", []).append(old)
+        b["workspace"] = torch.empty(max(need) + 256, dtype=torch.uint8, device=dev)
         return b
 
     def capture(self, T: int):

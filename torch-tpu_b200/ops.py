@@ -329,6 +329,20 @@ def _chk_accumulate(accumulate, t, name):
         raise ValueError(f"accumulate needs fp32 {name} to add to")
 
 
+def check_weight_grads(grads, names, shape, accumulate, device):
+    """Buffers of one call's weight gradients: fp32 or bf16, all of one type, fp32 to add to."""
+    for n, t in zip(names, grads):
+        _chk_grad(t, n, _GRAD, shape, device)
+        _chk_accumulate(accumulate, t, n)
+    if any(t.dtype != grads[0].dtype for t in grads):
+        raise ValueError(f"{', '.join(names)} must be of one dtype")
+
+
+def overlap(a, b):
+    """Whether two contiguous tensors share memory."""
+    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+
+
 _F32, _BF16, _I32, _E4M3 = (torch.float32,), (torch.bfloat16,), (torch.int32,), (torch.float8_e4m3fn,)
 _GRAD = (torch.float32, torch.bfloat16)
 
@@ -478,11 +492,7 @@ def experts_backward(dout, x, wg, wu, wd, sg, su, sd, ids, topk_w=None, *, dx=No
     if weight_grads is not None:
         if len(weight_grads) != 3:
             raise ValueError("weight_grads is (dwg, dwu, dwd)")
-        for n, t in zip(("dwg", "dwu", "dwd"), weight_grads):
-            _chk_grad(t, n, _GRAD, (E, I, H), dev)
-            _chk_accumulate(accumulate, t, n)
-        if len({t.dtype for t in weight_grads}) > 1:
-            raise ValueError("dwg, dwu and dwd must be of one dtype")
+        check_weight_grads(weight_grads, ("dwg", "dwu", "dwd"), (E, I, H), accumulate, dev)
     _chk_status(status, dev)
     with _on(dev):
         d = make_backward_desc(T, H, I, E, k, per_slot=per_slot, scale_dtype=sg.dtype,
