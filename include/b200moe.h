@@ -291,7 +291,8 @@ int b200moe_route_backward(float* dlogits, const float* logits, const float* log
 
 /* Of b200moe_router_logits: dx[T,H] (bf16) = dlogits[T,E] . wr[E,H], dwr[E,H] = dlogits^T . x[T,H].  dlogits fp32 (for dx
  * taken to 2^-17 relative, for dwr in full); dx or dwr may be NULL, and then wr or x too.  add_dx = 1 adds to what dx holds, e.g. the
- * experts' dx (the product is rounded to bf16 before the sum or with it).  H % 8 == 0, E <= 1024. */
+ * experts' dx (the product is rounded to bf16 before the sum or with it).  H % 8 == 0, E <= 1024.
+ * A workspace size of 1: these sizes need none, workspace may be NULL. */
 size_t b200moe_router_logits_backward_workspace_bytes(int64_t T, int64_t H, int64_t E);
 int b200moe_router_logits_backward(void* dx, int add_dx, void* dwr, int dwr_dtype, int accumulate, const float* dlogits,
                                    const void* x, const void* wr, int64_t T, int64_t H, int64_t E, void* workspace, size_t workspace_bytes,

@@ -539,8 +539,13 @@ struct RouterLayout {
   size_t split, part, total;
   int Ep, parts, stacked;  // stacked: dlogits' three numbers as one K range, else as rows of output
 };
+bool router_few(int64_t T, int64_t E) { return T <= RGS_MAX_T && T * E <= RGS_MAX_TE; }  // (one kernel, without a workspace)
 RouterLayout router_layout(int64_t T, int64_t H, int64_t E) {
   RouterLayout L{};
+  if (router_few(T, E)) {
+    L.total = 1;
+    return L;
+  }
   Carve w;
   L.Ep = (int)align_up((size_t)E, 64);
   // A tile is 256 x 256 outputs and 74 CTA pairs work at a time.  dlogits' three numbers are three times the output rows,
@@ -579,8 +584,7 @@ extern "C" int b200moe_router_logits_backward(void* dx, int add_dx, void* dwr, i
   MOE_CHECK_ARG(dlogits && (dx || dwr) && (!dx || wr) && (!dwr || x) && (!add_dx || dx));
   if ((dx && !(moe_aligned16(dx) && moe_aligned16(wr))) || (dwr && !(moe_aligned16(dwr) && moe_aligned16(x)))) return B200MOE_EALIGN;
   if (!moe_tc_available()) return B200MOE_EDRIVER;
-  const RouterLayout L = router_layout(T, H, E);
-  if (T <= RGS_MAX_T && T * E <= RGS_MAX_TE) {
+  if (router_few(T, E)) {
     const size_t smem = sizeof(float) * (size_t)(T * E + (dwr ? T * RGS_COLS : 0) + (dx ? E * RGS_COLS : 0));
     static bool attr_set[64] = {};
     int dev = 0;
@@ -595,6 +599,7 @@ extern "C" int b200moe_router_logits_backward(void* dx, int add_dx, void* dwr, i
                       reinterpret_cast<const __nv_bfloat16*>(dwr ? x : nullptr), reinterpret_cast<const __nv_bfloat16*>(wr), (int)T, (int)H,
                       (int)E);
   }
+  const RouterLayout L = router_layout(T, H, E);
   if (!workspace || workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return B200MOE_EWORKSPACE;
   char* ws = reinterpret_cast<char*>(workspace);
   __nv_bfloat16* split = reinterpret_cast<__nv_bfloat16*>(ws + L.split);

@@ -109,13 +109,14 @@ class FusedMoE:
         if shared_grads is not None and self.shared is None:
             raise ValueError("shared_grads without a shared expert")
         # (here, not in the calls below: nothing has been added to a buffer when another one is refused)
+        dev = self.w[0].get_device()
         if router_grad is not None:
-            ops.check_weight_grads([router_grad], ["router_grad"], self.router_w.shape, accumulate, self.device)
+            ops.check_weight_grads([router_grad], ["router_grad"], self.router_w.shape, accumulate, dev)
         for grads, weights, name in ((weight_grads, self.w, "weight_grads"), (shared_grads, self.shared, "shared_grads")):
             if grads is not None:
                 if len(grads) != 3:
                     raise ValueError(f"{name} is (dwg, dwu, dwd)")
-                ops.check_weight_grads(grads, [f"{name}[{i}]" for i in range(3)], weights[0].shape, accumulate, self.device)
+                ops.check_weight_grads(grads, [f"{name}[{i}]" for i in range(3)], weights[0].shape, accumulate, dev)
         b = self._backward_buffers(weight_grads is not None, shared_grads is not None)
         dx = b["dx"][:T] if dx is None else dx
         for n, t in (("x", x), ("dout", dout)):  # (both are read after dx's first store)

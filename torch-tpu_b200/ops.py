@@ -258,70 +258,83 @@ def linear_w8(x, w, scale, out=None, workspace=None, status=None):
 # Of the calls above.  Nothing here is an autograd function: a training loop calls them in reverse order, as
 # layer.FusedMoE.backward does.  All tensors of a call are on one device, which need not be the current one.
 
-def _chk_grad(t, name, dtypes, shape, device):
-    if (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == shape and t.device == device and device.type == "cuda"
-            and t.is_contiguous()):
+# (What a small call takes on the host is these checks, its outputs and the launch: devices are compared as numbers, outputs are made
+# like an input of their shape where there is one, and the stream's handle is asked for without a Stream object.)
+
+def _shape(t, name, dims):
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError(f"{name} must be a tensor of {dims} dimensions")
+    return t.shape
+
+
+def _lead(t, name, dims):
+    """The device's number and the shape of the tensor that the others are checked against."""
+    shape = _shape(t, name, dims)
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a contiguous CUDA tensor")
+    return t.get_device(), shape
+
+
+def _chk_grad(t, name, dtypes, shape, dev):
+    if isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype in dtypes and t.shape == shape and t.is_contiguous():
         return
     _chk(t, name)
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be on cuda:{dev}, got {t.device}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
     raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _grad_out(t, name, dtypes, shape, like):
+def _grad_out(t, name, dtypes, shape, like, dev):
     """`t`, checked, or a new tensor of the first of `dtypes`, on the device of `like`."""
-    device = like.device
-    if t is None:
-        return like.new_empty(shape) if like.dtype is dtypes[0] else like.new_empty(shape, dtype=dtypes[0])
-    _chk_grad(t, name, dtypes, shape, device)
-    return t
-
-
-def _rank(t, name, dims):
-    if not isinstance(t, torch.Tensor) or t.dim() != dims:
-        raise ValueError(f"{name} must be a tensor of {dims} dimensions")
+    if t is not None:
+        _chk_grad(t, name, dtypes, shape, dev)
+        return t
+    if like.dtype is dtypes[0] and like.shape == shape:
+        return torch.empty_like(like)
+    return like.new_empty(shape, dtype=dtypes[0])
 
 
 def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _on(device):
+def _on(dev):
     """The calls below launch on the current device: the tensors' one, for their time."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if dev == _current_device() else torch.cuda.device(dev)
 
 
 _HERE = contextlib.nullcontext()
-
-
-def _raw_stream(device):
-    """The current stream's handle (asked for without making a Stream object of it, which takes a sixth of a small call)."""
-    if _handle_of_stream is not None:
-        return _handle_of_stream(device.index)
-    return torch.cuda.current_stream(device).cuda_stream
-
-
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (a CUDA tensor was checked: CUDA is up)
 _handle_of_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _workspace(workspace, need, what, device):
+def _raw_stream(dev):
+    if _handle_of_stream is not None:
+        return _handle_of_stream(dev)
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _workspace(workspace, need, what, dev):
     if need == 0:
         raise ValueError(f"unsupported sizes for {what} (see include/b200moe.h)")
     if workspace is None:
-        workspace = torch.empty(need + 256, dtype=torch.uint8, device=device)
+        if need == 1:
+            return None, None, 0
+        workspace = torch.empty(need + 256, dtype=torch.uint8, device=dev)
     else:
         _chk(workspace, "workspace")
-        if workspace.device != device:
-            raise ValueError(f"workspace must be on {device}, got {workspace.device}")
-    base = (workspace.data_ptr() + 255) // 256 * 256
-    return workspace, base, workspace.numel() * workspace.element_size() - (base - workspace.data_ptr())
+        if workspace.get_device() != dev:
+            raise ValueError(f"workspace must be on cuda:{dev}, got {workspace.device}")
+    at = workspace.data_ptr()
+    base = (at + 255) // 256 * 256
+    return workspace, base, workspace.nbytes - (base - at)
 
 
-def _chk_status(status, device):
+def _chk_status(status, dev):
     if status is not None:
-        _chk_grad(status, "status", _I32, status.shape, device)
+        _chk_grad(status, "status", _I32, status.shape, dev)
 
 
 def _chk_accumulate(accumulate, t, name):
@@ -329,10 +342,10 @@ def _chk_accumulate(accumulate, t, name):
         raise ValueError(f"accumulate needs fp32 {name} to add to")
 
 
-def check_weight_grads(grads, names, shape, accumulate, device):
+def check_weight_grads(grads, names, shape, accumulate, dev):
     """Buffers of one call's weight gradients: fp32 or bf16, all of one type, fp32 to add to."""
     for n, t in zip(names, grads):
-        _chk_grad(t, n, _GRAD, shape, device)
+        _chk_grad(t, n, _GRAD, shape, dev)
         _chk_accumulate(accumulate, t, n)
     if any(t.dtype != grads[0].dtype for t in grads):
         raise ValueError(f"{', '.join(names)} must be of one dtype")
@@ -351,9 +364,8 @@ def route_backward(dw, logits, ids, score_func="softmax", renorm=True, scale=1.0
     """Gradient of ``route`` with respect to the logits: dlogits fp32 [T,E] from dw [T,k] (fp32 or bf16), the logits that
     were routed and the ids that came out.  Groups and the selection bias have no gradient; ``logit_bias`` has the sum of
     dlogits over the tokens.  Slots with an id outside [0,E) count for nothing.  ``dlogits`` may be ``logits`` itself."""
-    _rank(logits, "logits", 2)
-    _rank(ids, "ids", 2)
-    dev, (T, E), k = logits.device, logits.shape, ids.shape[1]
+    dev, (T, E) = _lead(logits, "logits", 2)
+    k = _shape(ids, "ids", 2)[1]
     _chk_grad(logits, "logits", _F32, (T, E), dev)
     _chk_grad(ids, "ids", _I32, (T, k), dev)
     _chk_grad(dw, "dw", _GRAD, (T, k), dev)
@@ -362,7 +374,7 @@ def route_backward(dw, logits, ids, score_func="softmax", renorm=True, scale=1.0
     if score_func not in ("softmax", "sigmoid"):
         raise ValueError(f"score_func must be softmax or sigmoid, got {score_func!r}")
     with _on(dev):
-        dlogits = _grad_out(dlogits, "dlogits", _F32, (T, E), logits)
+        dlogits = _grad_out(dlogits, "dlogits", _F32, (T, E), logits, dev)
         sf = L.SCORE_SOFTMAX if score_func == "softmax" else L.SCORE_SIGMOID
         L.check(L.lib().b200moe_route_backward(_addr(dlogits), _addr(logits), _addr(logit_bias), _addr(ids), _addr(dw), _DT[dw.dtype],
                                                T, E, k, sf, int(renorm), float(scale), _raw_stream(dev)), "b200moe_route_backward")
@@ -374,11 +386,10 @@ def router_logits_backward(dlogits, x=None, wr=None, dx=None, dwr=None, accumula
     """Gradients of ``router_logits``: (dx bf16 [T,H] = dlogits . wr, dwr [E,H] = dlogits^T . x).  Without ``wr`` dx is
     None, without ``x`` dwr is.  ``dwr`` is fp32 unless a bf16 tensor is given; ``accumulate`` adds to what it holds (fp32).  ``add_dx`` adds to what ``dx`` holds (the
     experts' dx, say)."""
-    _rank(dlogits, "dlogits", 2)
     if x is None and wr is None:
         raise ValueError("x or wr is needed")
-    _rank(x if x is not None else wr, "x" if x is not None else "wr", 2)
-    dev, (T, E), H = dlogits.device, dlogits.shape, (x if x is not None else wr).shape[1]
+    dev, (T, E) = _lead(dlogits, "dlogits", 2)
+    H = (_shape(x, "x", 2) if x is not None else _shape(wr, "wr", 2))[1]
     _chk_grad(dlogits, "dlogits", _F32, (T, E), dev)
     if x is not None:
         _chk_grad(x, "x", _BF16, (T, H), dev)
@@ -391,8 +402,8 @@ def router_logits_backward(dlogits, x=None, wr=None, dx=None, dwr=None, accumula
     with _on(dev):
         need = L.lib().b200moe_router_logits_backward_workspace_bytes(T, H, E)
         keep, base, avail = _workspace(workspace, need, "b200moe_router_logits_backward", dev)
-        dx = _grad_out(dx, "dx", _BF16, (T, H), wr) if wr is not None else None
-        dwr = _grad_out(dwr, "dwr", _GRAD, (E, H), dlogits) if x is not None else None
+        dx = _grad_out(dx, "dx", _BF16, (T, H), x if x is not None else wr, dev) if wr is not None else None
+        dwr = _grad_out(dwr, "dwr", _GRAD, (E, H), dlogits, dev) if x is not None else None
         L.check(L.lib().b200moe_router_logits_backward(_addr(dx), int(add_dx), _addr(dwr), _DT[dwr.dtype] if dwr is not None else L.F32,
                                                        int(accumulate and dwr is not None), _addr(dlogits), _addr(x), _addr(wr), T, H, E,
                                                        base, avail, _addr(status), _raw_stream(dev)), "b200moe_router_logits_backward")
@@ -403,16 +414,15 @@ def combine_backward(dout, y, w, ids=None, num_experts=0, dy=None, dw=None):
     """Gradients of ``combine``: (dy bf16 [T,k,H] = w[t,j] * dout[t], dw fp32 [T,k] = <dout[t], y[t,j]>).  With ``ids`` the
     slots whose expert id is outside [0, num_experts) give zeros and their rows of y are not read (``combine_indexed``
     masks them the same way).  ``dy`` may be ``y`` itself.  The gradient of ``add`` is dout."""
-    _rank(y, "y", 3)
-    dev, (T, k, H) = y.device, y.shape
+    dev, (T, k, H) = _lead(y, "y", 3)
     _chk_grad(y, "y", _BF16, (T, k, H), dev)
     _chk_grad(dout, "dout", _BF16, (T, H), dev)
     _chk_grad(w, "w", (torch.float32, torch.bfloat16, torch.float16), (T, k), dev)
     if ids is not None:
         _chk_grad(ids, "ids", _I32, (T, k), dev)
     with _on(dev):
-        dy = _grad_out(dy, "dy", _BF16, (T, k, H), y)
-        dw = _grad_out(dw, "dw", _F32, (T, k), y)
+        dy = _grad_out(dy, "dy", _BF16, (T, k, H), y, dev)
+        dw = _grad_out(dw, "dw", _F32, (T, k), w, dev)
         L.check(L.lib().b200moe_combine_backward(_addr(dy), _addr(dw), _addr(dout), _addr(y), _addr(w), _DT[w.dtype], _addr(ids), num_experts,
                                                  T, k, H, _raw_stream(dev)), "b200moe_combine_backward")
     return dy, dw
@@ -422,11 +432,10 @@ def linear_w8_backward(dy, x=None, w=None, scale=None, dx=None, dw=None, accumul
     """Gradients of ``linear_w8``: (dx bf16 [M,K] = Q(dy) . dequant(w), dw [N,K] = dy^T . x).  Q: e4m3 per row and 128
     columns, as the forward call quantises x.  Without ``w`` (and ``scale``) dx is None, without ``x`` dw is.  ``dw`` is fp32
     unless a bf16 tensor is given; ``accumulate`` adds to what it holds (fp32)."""
-    _rank(dy, "dy", 2)
     if x is None and w is None:
         raise ValueError("x or w is needed")
-    _rank(x if x is not None else w, "x" if x is not None else "w", 2)
-    dev, (M, N), K = dy.device, dy.shape, (x if x is not None else w).shape[1]
+    dev, (M, N) = _lead(dy, "dy", 2)
+    K = (_shape(x, "x", 2) if x is not None else _shape(w, "w", 2))[1]
     _chk_grad(dy, "dy", _BF16, (M, N), dev)
     if x is not None:
         _chk_grad(x, "x", _BF16, (M, K), dev)
@@ -439,8 +448,8 @@ def linear_w8_backward(dy, x=None, w=None, scale=None, dx=None, dw=None, accumul
         sdt = _DT[scale.dtype] if w is not None else L.F32
         need = L.lib().b200moe_linear_w8_backward_workspace_bytes(M, K, N, sdt)
         keep, base, avail = _workspace(workspace, need, "b200moe_linear_w8_backward", dev)
-        dx = _grad_out(dx, "dx", _BF16, (M, K), dy) if w is not None else None
-        dw = _grad_out(dw, "dw", _GRAD, (N, K), dy) if x is not None else None
+        dx = _grad_out(dx, "dx", _BF16, (M, K), x if x is not None else dy, dev) if w is not None else None
+        dw = _grad_out(dw, "dw", _GRAD, (N, K), dy, dev) if x is not None else None
         L.check(L.lib().b200moe_linear_w8_backward(_addr(dx), _addr(dw), _DT[dw.dtype] if dw is not None else L.F32,
                                                    int(accumulate and dw is not None), _addr(dy), _addr(x), _addr(w),
                                                    _addr(scale) if w is not None else None, sdt, M, K, N, base, avail,
@@ -467,10 +476,8 @@ def experts_backward(dout, x, wg, wu, wd, sg, su, sd, ids, topk_w=None, *, dx=No
     ``add`` bf16 [T,H] is added to dx (the router's or a shared expert's).  ``weight_grads`` = (dwg, dwu, dwd), tensors
     [E,I,H] of one dtype, bf16 or fp32, that receive the weights' gradients; ``accumulate`` adds to what they hold (fp32).
     bf16-weight experts have no gradient here."""
-    _rank(x, "x", 2)
-    _rank(wg, "wg", 3)
-    _rank(ids, "ids", 2)
-    dev, (T, H), (E, I, _), k = x.device, x.shape, wg.shape, ids.shape[1]
+    dev, (T, H) = _lead(x, "x", 2)
+    (E, I, _), k = _shape(wg, "wg", 3), _shape(ids, "ids", 2)[1]
     _chk_grad(x, "x", _BF16, (T, H), dev)
     _chk_grad(ids, "ids", _I32, (T, k), dev)
     for n, t in (("wg", wg), ("wu", wu), ("wd", wd)):
@@ -500,9 +507,9 @@ def experts_backward(dout, x, wg, wu, wd, sg, su, sd, ids, topk_w=None, *, dx=No
                                grad_dtype=weight_grads[0].dtype if weight_grads is not None else torch.float32,
                                accumulate=accumulate and weight_grads is not None)
         keep, base, avail = _workspace(workspace, experts_backward_workspace_bytes(d), "b200moe_experts_backward", dev)
-        dx = _grad_out(dx, "dx", _BF16, (T, H), x)
+        dx = _grad_out(dx, "dx", _BF16, (T, H), x, dev)
         if not per_slot:
-            dw = _grad_out(dw, "dw", _F32, (T, k), x)
+            dw = _grad_out(dw, "dw", _F32, (T, k), topk_w, dev)
         g = [_addr(t) for t in weight_grads] if weight_grads is not None else [None] * 3
         L.check(L.lib().b200moe_experts_backward(_addr(dx), _addr(dw), *g, _addr(dout), _addr(x), _addr(wg), _addr(wu), _addr(wd), _addr(sg),
                                                  _addr(su), _addr(sd), _addr(ids), _addr(topk_w), _addr(add), ctypes.byref(d), base, avail,
