@@ -286,6 +286,28 @@ def test_experts_backward_per_slot_bf16_scales_and_weights(ops, T, k):
     check_experts(ops, problem(T, 256, 256, 6, k, w_dtype=torch.bfloat16, scale_dtype=torch.bfloat16), torch.bfloat16)
 
 
+@pytest.mark.parametrize("H,I,per_slot,scale_dtype", [(1024, 1024, False, torch.float32), (1152, 1152, False, torch.bfloat16),
+                                                      (1024, 1152, True, torch.float32), (2176, 896, False, torch.float32)])
+def test_experts_backward_many_rows(ops, H, I, per_slot, scale_dtype):
+    check_experts(ops, problem(1800, H, I, 4, 2, per_slot=per_slot, scale_dtype=scale_dtype), torch.bfloat16)
+
+
+@pytest.mark.parametrize("counts", [(2560, 0, 1, 100), (256, 257, 2047, 256), (0, 0, 2816, 0), (1, 128, 129, 2558)])
+def test_experts_backward_many_rows_uneven(ops, counts):
+    """Experts that end before, at and behind the border of a second tile; dropped pairs behind them."""
+    T = 2816
+    ids = torch.full((T,), -1)
+    flat = torch.repeat_interleave(torch.arange(4), torch.tensor(counts))
+    ids[:len(flat)] = flat
+    ids = ids[torch.randperm(T, generator=torch.Generator().manual_seed(1))].view(T, 1)
+    p = problem(T, 1280, 1280, 4, 1, ids=ids)
+    dropped = len(flat) < T
+    first = check_experts(ops, p, torch.float32, bad=dropped)
+    again = run_experts(ops, p, torch.float32)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    assert all(torch.equal(a, b) for a, b in zip(first[2], again[2]))
+
+
 def test_experts_backward_uneven_loads(ops):
     """All rows on one expert, experts without rows, a tail of one row behind whole tiles."""
     T, k, E = 257, 2, 9

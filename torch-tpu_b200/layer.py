@@ -122,7 +122,8 @@ class FusedMoE:
         for n, t in (("x", x), ("dout", dout)):  # (both are read after dx's first store)
             if ops.overlap(dx, t):
                 raise ValueError(f"dx shares memory with {n}")
-        ids, w = self.route(x) if T else (self.ids[:0], self.topk_w[:0])
+        with ops._on(dev):  # (the calls below see to it themselves)
+            ids, w = self.route(x) if T else (self.ids[:0], self.topk_w[:0])
         if self.shared is not None:  # the shared expert is one expert that every token takes with weight 1
             ops.experts_backward(dout, x, *self.shared, b["zeros"][:T], b["ones"][:T], dx=dx, dw=b["shared_dw"][:T],
                                  weight_grads=shared_grads, accumulate=accumulate, workspace=b["workspace"], status=self.status)
